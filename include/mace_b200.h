@@ -458,6 +458,168 @@ int mb_minmax_f32(mb_context *ctx, const float *in, int64_t size,
 int mb_histogram_f32(mb_context *ctx, const float *in, int64_t size, float min_v,
                      float max_v, int bins, int32_t *host_counts);
 
+/* ---- Operators of a language model's decode step ---------------------------
+ * No counterparts in the reference, whose operator set ends at convolutional
+ * and recurrent networks.  They stand beside its MatMul, Softmax, Quantize and
+ * Dequantize and serve a transformer layer one token at a time: projections
+ * with 4-bit weights, rotary positions, attention over a paged key-value
+ * cache, and eviction from that cache.
+ *
+ * Element types (DT_FLOAT, DT_HALF and DT_BFLOAT16 of the reference): values of
+ * the 16-bit types are widened to fp32,
+ * every sum is kept in fp32, results are rounded once, to nearest even.
+ *
+ * All calls enqueue on the context's stream and may be captured into a graph
+ * (mb_graph_begin; run the sequence once uncaptured first, as ever).  Indices
+ * that lie in device memory (positions, slots, page tables, lengths) are read
+ * by the kernels: one outside its range reads and writes nothing there, and
+ * the next mb_stream_sync fails with MB_RUNTIME_ERROR ("an index in device
+ * memory is outside its range").
+ *
+ * Paged cache: two pools of pages, keys and values, each
+ *   [num_pages][kv_heads][page_size][head_dim]
+ * and a table [batch][max_pages] of int32 page numbers: slot j of sequence b
+ * lies in page table[b][j / page_size] at j % page_size.  Entries behind a
+ * sequence's last page are never read.  No offset is kept in 32 bits. */
+enum { MB_F32 = 0, MB_F16 = 1, MB_BF16 = 2 };
+
+/* Frequencies of rotary positions, a host function: freq[i] radians per
+ * position for pair i < rotary_dim / 2, and the factor on rotated values.
+ *   MB_ROPE_PLAIN    base^(-2i / rotary_dim)
+ *   MB_ROPE_LINEAR   divided by factor
+ *   MB_ROPE_BASE     base * factor^(rotary_dim / (rotary_dim - 2)) for base
+ *                    (rotary_dim >= 4): the slowest pair is slowed by factor
+ *   MB_ROPE_BANDS    with turns = original_length * freq / 2 pi: pairs of at
+ *                    least `high` turns stay, of at most `low` are divided by
+ *                    factor, those between are mixed linearly in turns
+ *   MB_ROPE_RAMP     the same ends, mixed linearly in i, between the (whole)
+ *                    pairs at which turns are `high` and `low`; the factor on
+ *                    rotated values is 0.1 ln(factor) + 1 (YaRN)
+ * The others give a magnitude of 1.  Computed and returned in 64 bits. */
+enum { MB_ROPE_PLAIN = 0, MB_ROPE_LINEAR = 1, MB_ROPE_BASE = 2, MB_ROPE_BANDS = 3, MB_ROPE_RAMP = 4 };
+int mb_rope_frequencies(int scaling, int64_t rotary_dim, double base,
+                        double factor, double original_length, double low,
+                        double high, double *host_freq, float *host_magnitude);
+
+/* Rotary positions on x [tokens][heads][head_dim], strides in elements, the
+ * dims of a head contiguous:
+ *   (a, b) -> magnitude * (a cos t - b sin t, a sin t + b cos t),
+ *   t = positions[token] * freq[i],
+ * where pair i is (x[2i], x[2i + 1]) if interleaved, else
+ * (x[i], x[i + rotary_dim / 2]).  Dims from rotary_dim on are copied.
+ * inverse turns the other way, which is the gradient with respect to x.  The
+ * angle is formed and reduced in 64 bits.  y == x with the same strides is
+ * allowed, other overlaps are not.  freq: device memory, rotary_dim / 2
+ * doubles. */
+int mb_rope(mb_context *ctx, const void *x, void *y, const int32_t *positions,
+            const double *freq, int64_t tokens, int64_t heads, int64_t head_dim,
+            int64_t rotary_dim, int64_t x_token_stride, int64_t x_head_stride,
+            int64_t y_token_stride, int64_t y_head_stride, int interleaved,
+            int inverse, float magnitude, int dtype);
+
+/* A step's way into the cache, in one pass: q [tokens][heads][head_dim] is
+ * rotated into q_out (q_out == q allowed, then with the same stride), k
+ * [tokens][kv_heads][head_dim] is rotated into k_cache and v copied into
+ * v_cache, token t into slot slots[t] of the pool (page slots[t] / page_size,
+ * row slots[t] % page_size).  A negative slot leaves its token out of the
+ * cache (padding of a batch); q is rotated all the same.  Token strides in
+ * elements, heads contiguous (q, k and v may be parts of one row).  Slots that
+ * are not negative must differ from one another; which of two tokens stays in
+ * a slot named twice is not defined. */
+int mb_rope_kv_append(mb_context *ctx, const void *q, void *q_out,
+                      const void *k, const void *v, void *k_cache,
+                      void *v_cache, const int32_t *positions,
+                      const int32_t *slots, const double *freq, int64_t tokens,
+                      int64_t heads, int64_t kv_heads, int64_t head_dim,
+                      int64_t rotary_dim, int64_t q_token_stride,
+                      int64_t q_out_token_stride, int64_t k_token_stride,
+                      int64_t v_token_stride, int64_t num_pages,
+                      int64_t page_size, int interleaved, float magnitude,
+                      int dtype);
+
+/* Attention of one new token per sequence over the paged cache.  q and out
+ * [batch][heads][head_dim], token strides in elements; kv head h serves query
+ * heads h * heads / kv_heads .. (h + 1) * heads / kv_heads - 1.
+ *   s_j = scale * q . k_j,  p_j = exp(s_j - lse),  out = sum_j p_j v_j
+ * over the slots j < lengths[b], or with window > 0 the last `window` of them.
+ * lse (may be NULL): [batch][heads].  A sequence of length 0 gives out = 0 and
+ * lse = -inf, and so does one whose every s_j is -inf.
+ * max_length is the longest that lengths may hold (a longer one, or one beyond
+ * the table, is an index outside its range: the slots up to max_length count);
+ * it sizes the grid, so a call that is captured into a graph and replayed as
+ * sequences grow names the longest of them all.
+ * weights_out (may be NULL): [batch][kv_heads][weights_stride] floats, slot j
+ * receives weights_in[j] (0 where weights_in is NULL; weights_in ==
+ * weights_out is allowed) plus the sum of p_j over the query heads that kv
+ * head h serves; slots outside the window receive weights_in alone, entries
+ * from lengths[b] on stay as they are.  head_dim up to 256. */
+int mb_paged_attention(mb_context *ctx, const void *q, const void *k_cache,
+                       const void *v_cache, const int32_t *page_table,
+                       const int32_t *lengths, void *out, float *lse,
+                       const float *weights_in, float *weights_out,
+                       int64_t batch, int64_t heads, int64_t kv_heads,
+                       int64_t head_dim, int64_t q_stride, int64_t out_stride,
+                       int64_t num_pages, int64_t page_size, int64_t max_pages,
+                       int64_t max_length, int64_t window,
+                       int64_t weights_stride, float scale, int dtype);
+
+/* Eviction from the cache by accumulated weight (mb_paged_attention's
+ * weights_out).  Each kv head of a sequence longer than `budget` keeps
+ * `budget` slots: the first `sinks`, the last `recent`, and of those between
+ * the ones with the largest weights (of equal weights the lower slots; NaN
+ * counts as less than everything).  A shorter sequence keeps all.  What is kept stays
+ * in order and is copied to slots 0, 1, ... of the destination: pages of
+ * k_dst / v_dst named by dst_table (the pools may be the source pools, the
+ * pages may not be pages that the call reads).  Device memory is written as
+ * follows, all of it only up to the new length min(lengths[b], budget):
+ *   dst_lengths [batch]                     the new lengths (may be lengths)
+ *   dst_weights [batch][kv_heads][budget]   the weights of the kept slots
+ *   kept        [batch][kv_heads][budget]   their old slots, ascending; here
+ *                                           entries from the new length on
+ *                                           become -1
+ * weights: [batch][kv_heads][weights_stride].  sinks + recent <= budget. */
+int mb_kv_evict(mb_context *ctx, const void *k_src, const void *v_src,
+                const int32_t *src_table, const int32_t *lengths,
+                const float *weights, void *k_dst, void *v_dst,
+                const int32_t *dst_table, int32_t *dst_lengths,
+                float *dst_weights, int32_t *kept, int64_t batch,
+                int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                int64_t src_pages, int64_t src_max_pages, int64_t dst_pages,
+                int64_t dst_max_pages, int64_t max_length,
+                int64_t weights_stride, int64_t budget, int64_t sinks,
+                int64_t recent, int dtype);
+
+/* 4-bit microscaled floating point (OCP MX, MXFP4): a row is cut into blocks
+ * of 32 values, each held as a shared power of two 2^(s - 127), s a byte
+ * (E8M0; 255 is NaN), and 32 codes of 4 bits (E2M1: a sign and 0, 0.5, 1, 1.5,
+ * 2, 3, 4, 6), packed low half first.
+ *   codes   [rows][ceil(cols / 32)][16] bytes; codes behind the last column
+ *           are 0
+ *   scales  tiles of 128 rows x 4 blocks, tile (r / 128, b / 4) row-major, in
+ *           each the byte of row r and block b at
+ *           (r % 32) * 16 + (r / 32 % 4) * 4 + b % 4
+ *           (what the tensor core takes); bytes of absent rows and blocks are
+ *           0.  mb_mxfp4_scale_bytes(rows, cols) bytes in all.
+ * Quantization: s - 127 = max(floor(log2 max|x|) - 2, -127), codes rounded to
+ * nearest even, saturated at 6; a block that holds an infinity or a NaN gets
+ * scale 255 and codes 0.  x: rows of `stride` elements. */
+size_t mb_mxfp4_scale_bytes(int64_t rows, int64_t cols);
+int mb_quantize_mxfp4(mb_context *ctx, const void *x, uint8_t *codes,
+                      uint8_t *scales, int64_t rows, int64_t cols,
+                      int64_t stride, int dtype);
+int mb_dequantize_mxfp4(mb_context *ctx, const uint8_t *codes,
+                        const uint8_t *scales, void *x, int64_t rows,
+                        int64_t cols, int64_t stride, int dtype);
+
+/* C[m][n] = sum_k A[m][k] B[n][k] (+ bias[n]), A [M][K] and B [N][K] both in
+ * MXFP4 as above, bias fp32 (may be NULL), C in rows of `stride` elements of
+ * the given type.  Products are exact, sums fp32.  codes and scales 16-byte
+ * aligned. */
+int mb_gemm_mxfp4(mb_context *ctx, const uint8_t *a_codes,
+                  const uint8_t *a_scales, const uint8_t *b_codes,
+                  const uint8_t *b_scales, const float *bias, void *C,
+                  int64_t M, int64_t N, int64_t K, int64_t stride, int dtype);
+
 /* ---- The pixels a strided 1x1 convolution reads, gathered once.  No operator
  * of its own in the reference: arm::Conv2dGeneral / ref::Conv2d index the input
  * with the stride (mace/ops/ref/conv_2d.cc:36-122).  A 1x1 convolution with

@@ -7,6 +7,10 @@ import subprocess
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _LIB = os.path.join(_HERE, "libmace_b200.so")
 
+# element types of the decode-step operators, scalings of rotary frequencies (include/mace_b200.h)
+F32, F16, BF16 = 0, 1, 2
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_BANDS, ROPE_RAMP = range(5)
+
 STATUS = {0: "MACE_SUCCESS", 1: "MACE_INVALID_ARGS", 2: "MACE_OUT_OF_RESOURCES",
           3: "MACE_UNSUPPORTED", 4: "MACE_RUNTIME_ERROR"}
 
@@ -103,6 +107,15 @@ PROTOTYPES = {
     "mb_gemm_u8_static_scratch": (_int, [_vp] * 5 + [_int] + [_i64] * 3 + [_int] * 2 +
                                   [_i32] * 5 + [_int, C.c_char_p, _sz]),
     "mb_gemm_u8_static_scratch_status": (_int, [_vp, C.POINTER(_int)]),
+    "mb_rope_frequencies": (_int, [_int, _i64] + [C.c_double] * 5 + [C.POINTER(C.c_double), C.POINTER(_f32)]),
+    "mb_rope": (_int, [_vp] * 5 + [_i64] * 8 + [_int] * 2 + [_f32, _int]),
+    "mb_rope_kv_append": (_int, [_vp] * 10 + [_i64] * 11 + [_int, _f32, _int]),
+    "mb_paged_attention": (_int, [_vp] * 10 + [_i64] * 12 + [_f32, _int]),
+    "mb_kv_evict": (_int, [_vp] * 12 + [_i64] * 13 + [_int]),
+    "mb_mxfp4_scale_bytes": (_sz, [_i64] * 2),
+    "mb_quantize_mxfp4": (_int, [_vp] * 4 + [_i64] * 3 + [_int]),
+    "mb_dequantize_mxfp4": (_int, [_vp] * 4 + [_i64] * 3 + [_int]),
+    "mb_gemm_mxfp4": (_int, [_vp] * 7 + [_i64] * 4 + [_int]),
     "mb_histogram_f32": (_int, [_vp, _vp, _i64, _f32, _f32, _int, C.POINTER(_i32)]),
     "mb_set_runtime_failure_ratio": (_int, [_f32]),
     "mb_should_mock_runtime_failure": (_int, []),
@@ -387,3 +400,65 @@ class Context:
         self._check(_ops.mb_avgpool_u8_nhwc(self._p,
             x.ptr, out.ptr, N, H, W, Cc, kernel[0], kernel[1], strides[0], strides[1],
             pad_tl[0], pad_tl[1], out_hw[0], out_hw[1]))
+
+    def rope(self, x, y, positions, freq, tokens, heads, head_dim, rotary_dim, dtype, x_strides=None, y_strides=None,
+             interleaved=False, inverse=False, magnitude=1.0):
+        """Strides: (token, head) in elements; heads of head_dim side by side where not given."""
+        xs, ys = x_strides or (heads * head_dim, head_dim), y_strides or (heads * head_dim, head_dim)
+        self._check(_ops.mb_rope(self._p, x.ptr, y.ptr, positions.ptr, freq.ptr, tokens, heads, head_dim, rotary_dim,
+                                 xs[0], xs[1], ys[0], ys[1], int(interleaved), int(inverse), magnitude, dtype))
+
+    def rope_kv_append(self, q, q_out, k, v, k_cache, v_cache, positions, slots, freq, tokens, heads, kv_heads, head_dim,
+                       rotary_dim, num_pages, page_size, dtype, token_strides=None, q_out_stride=None, interleaved=False,
+                       magnitude=1.0):
+        """token_strides: of q, k and v, in elements; each side by side where not given."""
+        st = token_strides or (heads * head_dim, kv_heads * head_dim, kv_heads * head_dim)
+        self._check(_ops.mb_rope_kv_append(self._p, q.ptr, q_out.ptr, k.ptr, v.ptr, k_cache.ptr, v_cache.ptr,
+            positions.ptr, slots.ptr, freq.ptr, tokens, heads, kv_heads, head_dim, rotary_dim, st[0],
+            heads * head_dim if q_out_stride is None else q_out_stride, st[1], st[2], num_pages, page_size,
+            int(interleaved), magnitude, dtype))
+
+    def paged_attention(self, q, k_cache, v_cache, page_table, lengths, out, batch, heads, kv_heads, head_dim, num_pages,
+                        page_size, max_pages, max_length, scale, dtype, lse=None, weights_in=None, weights_out=None,
+                        weights_stride=0, window=0, q_stride=None, out_stride=None):
+        self._check(_ops.mb_paged_attention(self._p, q.ptr, k_cache.ptr, v_cache.ptr, page_table.ptr, lengths.ptr,
+            out.ptr, lse.ptr if lse is not None else None, weights_in.ptr if weights_in is not None else None,
+            weights_out.ptr if weights_out is not None else None, batch, heads, kv_heads, head_dim,
+            heads * head_dim if q_stride is None else q_stride, heads * head_dim if out_stride is None else out_stride,
+            num_pages, page_size, max_pages, max_length, window, weights_stride, scale, dtype))
+
+    def kv_evict(self, k_src, v_src, src_table, lengths, weights, k_dst, v_dst, dst_table, dst_lengths, dst_weights, kept,
+                 batch, kv_heads, head_dim, page_size, src_pages, src_max_pages, dst_pages, dst_max_pages, max_length,
+                 weights_stride, budget, sinks, recent, dtype):
+        self._check(_ops.mb_kv_evict(self._p, k_src.ptr, v_src.ptr, src_table.ptr, lengths.ptr, weights.ptr, k_dst.ptr,
+            v_dst.ptr, dst_table.ptr, dst_lengths.ptr, dst_weights.ptr, kept.ptr, batch, kv_heads, head_dim, page_size,
+            src_pages, src_max_pages, dst_pages, dst_max_pages, max_length, weights_stride, budget, sinks, recent, dtype))
+
+    def quantize_mxfp4(self, x, codes, scales, rows, cols, dtype, stride=None):
+        self._check(_ops.mb_quantize_mxfp4(self._p, x.ptr, codes.ptr, scales.ptr, rows, cols,
+                                           cols if stride is None else stride, dtype))
+
+    def dequantize_mxfp4(self, codes, scales, x, rows, cols, dtype, stride=None):
+        self._check(_ops.mb_dequantize_mxfp4(self._p, codes.ptr, scales.ptr, x.ptr, rows, cols,
+                                             cols if stride is None else stride, dtype))
+
+    def gemm_mxfp4(self, a_codes, a_scales, b_codes, b_scales, Cout, M, N, K, dtype, bias=None, stride=None):
+        """C = A B^T (+ bias): A [M][K] and B [N][K] in MXFP4."""
+        self._check(_ops.mb_gemm_mxfp4(self._p, a_codes.ptr, a_scales.ptr, b_codes.ptr, b_scales.ptr,
+                                       bias.ptr if bias is not None else None, Cout.ptr, M, N, K,
+                                       N if stride is None else stride, dtype))
+
+
+def rope_frequencies(rotary_dim, base=10000.0, scaling=ROPE_PLAIN, factor=1.0, original_length=0.0, low=1.0, high=32.0):
+    """(numpy float64 [rotary_dim / 2], magnitude): mb_rope_frequencies, a host function."""
+    import numpy as np
+    freq, magnitude = np.zeros(max(rotary_dim // 2, 1)), _f32()
+    st = lib().mb_rope_frequencies(scaling, rotary_dim, base, factor, original_length, low, high,
+                                   freq.ctypes.data_as(C.POINTER(C.c_double)), C.byref(magnitude))
+    if st != 0:
+        raise MaceB200Error(st, "mb_rope_frequencies: bad scaling, size or factor")
+    return freq[:rotary_dim // 2], float(magnitude.value)
+
+
+def mxfp4_scale_bytes(rows, cols):
+    return int(lib().mb_mxfp4_scale_bytes(rows, cols))

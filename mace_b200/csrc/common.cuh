@@ -22,6 +22,7 @@ enum : int {
   MB_DEV_TIMEOUT_PRODUCER = 1,
   MB_DEV_TIMEOUT_MMA = 2,
   MB_DEV_TIMEOUT_EPILOGUE = 3,
+  MB_DEV_BAD_INDEX = 4,  // not a wait: an index in device memory outside its range (elements.cuh)
 };
 
 struct mb_context {
@@ -52,6 +53,13 @@ struct mb_context {
   bool f32_stem_smem[4] = {false, false, false, false};  // its kernels whose shared-memory limit was raised
   int f32_rows = 0;            // gemm_f32_rows.cu: 0 by rule, 1 never, 2 wherever it can run
   bool f32_rows_smem[2] = {false, false};  // its kernels whose shared-memory limit was raised
+  // Partial results of the decode-step operators, and their arrival counters (zero between calls).  Both grow outside graph
+  // captures only; blocks that a recorded graph may refer to are kept until the context ends.
+  void *op_scratch = nullptr, *op_counters = nullptr;
+  size_t op_scratch_bytes = 0, op_counters_bytes = 0;
+  std::vector<void *> op_kept;
+  uint32_t attention_attr_mask = 0;  // kernels of paged_attention.cu whose shared-memory limit was raised
+  uint32_t mxfp4_attr_mask = 0;      // the same for gemm_mxfp4.cu
   uint32_t f32_pairs_attr_mask = 0;  // kernels of gemm_f32_pairs.cu whose shared-memory limit was raised
   int *dev_status = nullptr;   // status word of bounded-wait failures: the device's address of host_status
   int *host_status = nullptr;  // the word itself, in page-locked host memory: read there at sync
@@ -134,6 +142,10 @@ int mb_scratch(mb_context *ctx, size_t bytes, void **ptr);
 // null where there is no memory: the caller then does without.  Never freed before the context once a graph may refer to it.
 constexpr size_t WEIGHT_SCRATCH_BYTES = 256u << 20;  // what is asked of it at most
 int mb_weight_scratch(mb_context *ctx, size_t bytes, void **ptr);
+
+// Two more for the decode-step operators: contents do not survive the call, and counters that are zero before and after it.
+int mb_op_scratch(mb_context *ctx, size_t bytes, void **ptr);
+int mb_op_counters(mb_context *ctx, size_t count, unsigned **ptr);
 
 // ---- programmatic dependent launch ------------------------------------------------------------
 // A kernel launched through mb_launch_chained may be started before the kernel in front of it in

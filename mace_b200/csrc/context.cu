@@ -81,6 +81,53 @@ int mb_weight_scratch(mb_context *ctx, size_t bytes, void **ptr) {
   return MB_SUCCESS;
 }
 
+static int grow_kept(mb_context *ctx, size_t bytes, void **block, size_t *have, bool zeroed) {
+  if (bytes <= *have) return MB_SUCCESS;
+  if (ctx->capturing)
+    return mb_fail(ctx, MB_RUNTIME_ERROR, "scratch arena would grow during graph capture; run the sequence once first");
+  if (mb_should_mock_runtime_failure())
+    return mb_fail(ctx, MB_OUT_OF_RESOURCES, "scratch arena: mock runtime failure (MACE_RUNTIME_FAILURE_RATIO)");
+  if (*block != nullptr) {
+    if (ctx->captured_any) {
+      try {
+        ctx->op_kept.push_back(*block);
+      } catch (...) {
+        return mb_fail(ctx, MB_OUT_OF_RESOURCES, "scratch arena: no host memory");
+      }
+    } else {
+      MB_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
+      MB_CUDA(ctx, cudaFree(*block));
+    }
+    *block = nullptr;
+    *have = 0;
+  }
+  const size_t want = align_up(bytes + bytes / 4, 1 << 16);
+  void *fresh = nullptr;
+  MB_CUDA(ctx, cudaMalloc(&fresh, want));
+  if (zeroed) {
+    const int st = mb_check_cuda(ctx, cudaMemsetAsync(fresh, 0, want, ctx->stream), "cudaMemsetAsync");
+    if (st != MB_SUCCESS) {
+      cudaFree(fresh);
+      return st;
+    }
+  }
+  *block = fresh;
+  *have = want;
+  return MB_SUCCESS;
+}
+
+int mb_op_scratch(mb_context *ctx, size_t bytes, void **ptr) {
+  MB_RETURN_IF_ERROR(grow_kept(ctx, bytes, &ctx->op_scratch, &ctx->op_scratch_bytes, false));
+  *ptr = ctx->op_scratch;
+  return MB_SUCCESS;
+}
+
+int mb_op_counters(mb_context *ctx, size_t count, unsigned **ptr) {
+  MB_RETURN_IF_ERROR(grow_kept(ctx, count * sizeof(unsigned), &ctx->op_counters, &ctx->op_counters_bytes, true));
+  *ptr = static_cast<unsigned *>(ctx->op_counters);
+  return MB_SUCCESS;
+}
+
 namespace {
 
 // Results to page-locked host memory, by a kernel that writes there itself: behind other kernels of a stream the copy engine
@@ -195,6 +242,9 @@ int mb_destroy(mb_context *ctx) {
   if (ctx->weight_scratch) cudaFree(ctx->weight_scratch);
   for (void *block : ctx->weight_scratch_kept) cudaFree(block);
   if (ctx->skinny_ws) cudaFree(ctx->skinny_ws);
+  if (ctx->op_scratch) cudaFree(ctx->op_scratch);
+  if (ctx->op_counters) cudaFree(ctx->op_counters);
+  for (void *block : ctx->op_kept) cudaFree(block);
   if (ctx->host_status) cudaFreeHost(ctx->host_status);
   if (ctx->stream) cudaStreamDestroy(ctx->stream);
   delete ctx;
@@ -397,6 +447,8 @@ int mb_stream_sync(mb_context *ctx) {
   const int code = *static_cast<volatile int *>(ctx->host_status);
   if (code != 0) {
     *static_cast<volatile int *>(ctx->host_status) = 0;
+    if (code == MB_DEV_BAD_INDEX)
+      return mb_fail(ctx, MB_RUNTIME_ERROR, "an index in device memory is outside its range (page, slot or length)");
     return mb_fail(ctx, MB_RUNTIME_ERROR,
                    "a kernel gave up a bounded wait (device status %d)", code);
   }

@@ -75,6 +75,13 @@ PyMethodDef kMethods[] = {
     MB_ENTRY(mb_dequantize_f32),
     MB_ENTRY(mb_transpose2d_batched),
     MB_ENTRY(mb_subsample_f32_nchw),
+    MB_ENTRY(mb_rope),
+    MB_ENTRY(mb_rope_kv_append),
+    MB_ENTRY(mb_paged_attention),
+    MB_ENTRY(mb_kv_evict),
+    MB_ENTRY(mb_quantize_mxfp4),
+    MB_ENTRY(mb_dequantize_mxfp4),
+    MB_ENTRY(mb_gemm_mxfp4),
     MB_ENTRY(mb_stream_sync),
     {nullptr, nullptr, 0, nullptr},
 };
