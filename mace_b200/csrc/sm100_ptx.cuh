@@ -502,6 +502,34 @@ __device__ __forceinline__ void mma_commit_elect(uint32_t bar) {
       : "memory");
 }
 
+// D[tmem] (+)= A[smem] * B[smem], 4-bit E2M1 inputs in blocks of 32 with E8M0 scales in tensor memory, fp32 accumulation.  Called by a
+// whole warp like the half-precision forms above.
+__device__ __forceinline__ void mma_mxf4_ss_elect(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scale_tmem,
+                                                  uint32_t b_scale_tmem, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred e, p;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+      "}\n"
+      :
+      : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scale_tmem), "r"(b_scale_tmem), "r"(accumulate)
+      : "memory");
+}
+
+// 512 bytes of shared memory (32 rows of 16) to four columns of tensor memory: row r to lane r of every 32 lanes.  Executed in
+// order with the MMAs that the same thread issues behind it.
+__device__ __forceinline__ void tmem_cp_32x128b_elect(uint32_t taddr, uint64_t smem_desc) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t"
+      "}\n" ::"r"(taddr), "l"(smem_desc)
+      : "memory");
+}
+
 // 16 consecutive 32-bit columns of this warp's 32 TMEM lanes <- one register per column.
 __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -628,6 +656,14 @@ __host__ __device__ constexpr uint32_t make_idesc(uint32_t c_fmt, uint32_t a_fmt
   return (c_fmt << 4) | (a_fmt << 7) | (b_fmt << 10) |
          (static_cast<uint32_t>(a_mn_major) << 15) |
          (static_cast<uint32_t>(b_mn_major) << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+// Instruction descriptor of kind::mxf4 (E2M1 inputs, E8M0 scales, K = 64, both operands K-major):
+//  [4,6) B's scale byte (0 or 2)   [7,10) A format   [10,12) B format (1 = E2M1)   [17,23) N >> 3   [23] scales are E8M0
+//  [24,29) M >> 4   [29,31) A's scale byte
+// A row's two scales are the bytes named here of its 32-bit word of tensor memory: row r in lane r % 32, column r / 32.
+__host__ __device__ constexpr uint32_t make_idesc_mxf4(uint32_t m, uint32_t n, uint32_t scale_byte) {
+  return (scale_byte << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((m >> 4) << 24) | (scale_byte << 29);
 }
 
 }  // namespace sm100
