@@ -318,6 +318,256 @@ __global__ void __launch_bounds__(THREADS) paged_attention_kernel(const Attentio
   finish<T, R>(p, at, WARPS, DIM, top_s, sum_s, acc_s, coef, total);
 }
 
+// ---- on the tensor cores: 16-bit types, rows of whole 16-byte words -----------------------------------------------------------
+//
+// Up to 16 query heads are the rows of mma.sync m16n8k16 (a decode step has no 128 rows for tcgen05 to multiply, and the cache's bytes
+// bound it by far: 16 rows cost 16 operations a byte where 250 would be needed).  Every warp has a ring of its own in shared
+// memory that its cp.asyncs fill with CHUNK slots' keys and values at a time, two stages ahead, so that no barrier joins warps
+// before the end.  Rows are swizzled in 16-byte words for ldmatrix.  Probabilities are multiplied as two 16-bit values, hi + lo:
+// their sum is the fp32 one to 2^-16 (bf16) or 2^-22, and the second product costs nothing that the memory does not hide.
+
+template <typename T> struct Mma;
+template <> struct Mma<__half> {
+  static __device__ __forceinline__ void run(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ void split(float x, float y, uint32_t &hi, uint32_t &lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+  }
+};
+template <> struct Mma<__nv_bfloat16> {
+  static __device__ __forceinline__ void run(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ void split(float x, float y, uint32_t &hi, uint32_t &lo) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    const float2 f = __bfloat1622float2(h);
+    const __nv_bfloat162 l = __floats2bfloat162_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+  }
+};
+
+template <bool TRANS>
+__device__ __forceinline__ void load_matrices(uint32_t addr, uint32_t (&r)[4]) {
+  if (TRANS)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+template <int DIM>
+struct Ring {
+  static constexpr int CHUNK = DIM == 64 ? 32 : 16;         // slots
+  static constexpr int ROW = DIM * 2, WORDS = DIM / 8;      // bytes of a row, its 16-byte words
+  static constexpr int PART = CHUNK * ROW, STAGE = 2 * PART;  // keys, then values
+  static constexpr int STAGES = 3;
+  static constexpr int BYTES = WARPS * STAGES * STAGE;
+  static constexpr int PITCH = DIM + 4;                     // floats between rows of the accumulators at the end
+  static_assert(WARPS * 16 * PITCH * 4 <= BYTES, "accumulators reuse the ring");
+};
+
+template <typename T, int DIM>
+__global__ void __launch_bounds__(THREADS) paged_attention_mma_kernel(const AttentionParams p) {
+  using G = Ring<DIM>;
+  constexpr int R = 16, CHUNK = G::CHUNK, KEY_TILES = CHUNK / 8, DIM_STEPS = DIM / 16, STAGES = G::STAGES;
+  extern __shared__ __align__(1024) uint8_t ring[];
+  __shared__ unsigned valid[WARPS][STAGES];
+  __shared__ float top_s[WARPS * R], sum_s[WARPS * R], coef[WARPS * R], total[2 * R];
+  mb_grid_dep_launch();
+  mb_grid_dep_wait();
+  const Place at(p, R);
+  if (at.split >= at.active) return;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = lane / 4, pair = lane % 4;
+  const T *k = static_cast<const T *>(p.k), *v = static_cast<const T *>(p.v);
+  const int32_t *table = p.table + static_cast<int64_t>(at.batch) * p.max_pages;
+  const uint32_t mine = sm100::smem_u32(ring) + warp * STAGES * G::STAGE;
+
+  // the queries of rows `row` and `row` + 8
+  uint32_t q[DIM_STEPS][4];
+#pragma unroll
+  for (int s = 0; s < DIM_STEPS; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int h = row + i % 2 * 8, d = s * 16 + i / 2 * 8 + pair * 2;
+      elem::Vec<T, 2> two;
+      two.word = 0;
+      if (h < at.heads && d < p.dim) {
+        const T *src = static_cast<const T *>(p.q) + at.batch * p.q_stride + static_cast<int64_t>(at.head0 + h) * p.dim + d;
+        two.v[0] = mb_load(src);
+        two.v[1] = mb_load(src + 1);
+      }
+      q[s][i] = two.word;
+    }
+  float acc[2 * DIM_STEPS][4], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 2 * DIM_STEPS; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+
+  const int chunks = (at.end - at.begin + CHUNK - 1) / CHUNK;   // of all warps; this one has warp, warp + WARPS, ..
+  const auto offset_of = [&](int chunk) -> int64_t {
+    const int slot = at.begin + chunk * CHUNK + lane;
+    return lane < CHUNK && chunk < chunks && slot < at.end ? slot_offset(p, table, at.kv_head, slot) : -1;
+  };
+  // `where`: lane l's offset of the chunk's slot l
+  const auto fetch = [&](int chunk, int stage, int64_t where) {
+    if (chunk < chunks) {
+      const unsigned ok = __ballot_sync(0xffffffffu, where >= 0);
+      if (lane == 0) valid[warp][stage] = ok;
+      const int word = lane % G::WORDS;
+#pragma unroll
+      for (int i = 0; i < CHUNK * G::WORDS / 32; ++i) {
+        const int r = i * (32 / G::WORDS) + lane / G::WORDS;
+        const int64_t from = __shfl_sync(0xffffffffu, where, r);
+        const bool there = from >= 0 && word * 8 < p.dim;
+        const int64_t src = there ? from + word * 8 : 0;
+        const uint32_t dst = mine + stage * G::STAGE + r * G::ROW + ((word ^ (r & 7)) << 4);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(k + src), "r"(there ? 16 : 0) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + G::PART), "l"(v + src), "r"(there ? 16 : 0) : "memory");
+      }
+    }
+    sm100::cp_async_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) fetch(warp + s * WARPS, s, offset_of(warp + s * WARPS));
+  int64_t ahead = offset_of(warp + (STAGES - 1) * WARPS);
+
+  int stage = 0;
+  for (int chunk = warp; chunk < chunks; chunk += WARPS) {
+    sm100::cp_async_wait<STAGES - 2>();
+    __syncwarp();
+    fetch(chunk + (STAGES - 1) * WARPS, stage == 0 ? STAGES - 1 : stage - 1, ahead);
+    ahead = offset_of(chunk + STAGES * WARPS);
+    const uint32_t keys = mine + stage * G::STAGE, values = keys + G::PART;
+    const unsigned ok = valid[warp][stage];
+    float s[KEY_TILES][4];
+#pragma unroll
+    for (int t = 0; t < KEY_TILES; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[t][j] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DIM_STEPS; ++d)
+#pragma unroll
+      for (int t = 0; t < KEY_TILES; t += 2) {
+        uint32_t b[4];
+        const int r = t * 8 + lane % 8 + lane / 16 * 8, word = 2 * d + lane / 8 % 2;
+        load_matrices<false>(keys + r * G::ROW + ((word ^ (r & 7)) << 4), b);
+        Mma<T>::run(s[t], q[d], b[0], b[1]);
+        Mma<T>::run(s[t + 1], q[d], b[2], b[3]);
+      }
+    const int slot = at.begin + chunk * CHUNK + pair * 2;
+    float m[2] = {top[0], top[1]};
+#pragma unroll
+    for (int t = 0; t < KEY_TILES; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[t][j] = (ok >> (t * 8 + pair * 2 + j % 2) & 1u) != 0 ? s[t][j] * p.scale2 : -INFINITY;
+        m[j / 2] = fmaxf(m[j / 2], s[t][j]);
+      }
+    if (p.logits != nullptr) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (row + 8 * h < at.heads) {
+          float *to = p.logits + (static_cast<int64_t>(at.batch) * p.heads + at.head0 + row + 8 * h) * p.logits_stride + slot;
+#pragma unroll
+          for (int t = 0; t < KEY_TILES; ++t)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              if (slot + t * 8 + j < at.end) to[t * 8 + j] = s[t][2 * h + j];
+        }
+    }
+    bool grew = false;
+    float back[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      m[h] = fmaxf(m[h], __shfl_xor_sync(0xffffffffu, m[h], 1));
+      m[h] = fmaxf(m[h], __shfl_xor_sync(0xffffffffu, m[h], 2));
+      grew = grew || m[h] != top[h];
+      const float safe = m[h] == -INFINITY ? 0.f : m[h];
+      back[h] = exp2f(top[h] - safe);
+      top[h] = m[h];
+      m[h] = safe;
+      sum[h] *= back[h];
+    }
+    if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+      for (int i = 0; i < 2 * DIM_STEPS; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] *= back[j / 2];
+    }
+#pragma unroll
+    for (int t = 0; t < KEY_TILES; t += 2) {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float x = exp2f(s[t + u][2 * h] - m[h]), y = exp2f(s[t + u][2 * h + 1] - m[h]);
+          sum[h] += x + y;
+          Mma<T>::split(x, y, hi[2 * u + h], lo[2 * u + h]);
+        }
+#pragma unroll
+      for (int d = 0; d < DIM_STEPS; ++d) {
+        uint32_t b[4];
+        const int r = t * 8 + lane % 16, word = 2 * d + lane / 16;
+        load_matrices<true>(values + r * G::ROW + ((word ^ (r & 7)) << 4), b);
+        Mma<T>::run(acc[2 * d], hi, b[0], b[1]);
+        Mma<T>::run(acc[2 * d + 1], hi, b[2], b[3]);
+        Mma<T>::run(acc[2 * d], lo, b[0], b[1]);
+        Mma<T>::run(acc[2 * d + 1], lo, b[2], b[3]);
+      }
+    }
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+  }
+  sm100::cp_async_wait<0>();
+  __syncthreads();
+  float *acc_s = reinterpret_cast<float *>(ring);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+    sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+    if (row + 8 * h < at.heads) {
+      const int r = warp * R + row + 8 * h;
+      if (pair == 0) {
+        top_s[r] = top[h];
+        sum_s[r] = sum[h];
+      }
+#pragma unroll
+      for (int i = 0; i < 2 * DIM_STEPS; ++i)
+        *reinterpret_cast<float2 *>(acc_s + r * G::PITCH + i * 8 + pair * 2) = make_float2(acc[i][2 * h], acc[i][2 * h + 1]);
+    }
+  }
+  __syncthreads();
+  finish<T, R>(p, at, WARPS, G::PITCH, top_s, sum_s, acc_s, coef, total);
+}
+
+template <typename T, int DIM>
+int launch_mma(mb_context *ctx, const AttentionParams &p, unsigned grid, int index) {
+  const auto kern = paged_attention_mma_kernel<T, DIM>;
+  if (!(ctx->attention_attr_mask & (1u << index))) {
+    MB_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<DIM>::BYTES));
+    ctx->attention_attr_mask |= 1u << index;
+  }
+  MB_CUDA(ctx, mb_launch_chained(ctx, kern, dim3(grid), dim3(THREADS), Ring<DIM>::BYTES, p));
+  return MB_SUCCESS;
+}
+
+template <typename T>
+int launch_mma(mb_context *ctx, const AttentionParams &p, unsigned grid, int index) {
+  if (p.dim <= 64) return launch_mma<T, 64>(ctx, p, grid, index);
+  if (p.dim <= 128) return launch_mma<T, 128>(ctx, p, grid, index + 1);
+  return launch_mma<T, 256>(ctx, p, grid, index + 2);
+}
+
 // What each slot has received of the query heads' probabilities, on top of what it had.
 __global__ void __launch_bounds__(256) attention_weights_kernel(const AttentionParams p, int chunks) {
   mb_grid_dep_launch();
@@ -386,7 +636,8 @@ extern "C" int mb_paged_attention(mb_context *ctx, const void *q, const void *k_
   p.scale2 = scale * LOG2E;
   p.status = ctx->dev_status;
 
-  const int rows = p.group >= 5 ? 8 : p.group >= 3 ? 4 : p.group;
+  const bool by_mma = dtype != MB_F32 && ctx->use_tensor_cores && head_dim % 8 == 0 && kv::aligned(k_cache, 16) && kv::aligned(v_cache, 16);
+  const int rows = by_mma ? 16 : p.group >= 5 ? 8 : p.group >= 3 ? 4 : p.group;
   p.blocks = (p.group + rows - 1) / rows;
   const int64_t units = batch * kv_heads * p.blocks;
   cut_runs(ctx, p, units);
@@ -414,7 +665,10 @@ extern "C" int mb_paged_attention(mb_context *ctx, const void *q, const void *k_
   }
   const unsigned grid = static_cast<unsigned>(units * p.splits);
   cudaError_t e = cudaSuccess;
-  MB_FOR_ELEMENT(dtype, {
+  if (by_mma) {
+    if (dtype == MB_F16) MB_RETURN_IF_ERROR(launch_mma<__half>(ctx, p, grid, 0));
+    else MB_RETURN_IF_ERROR(launch_mma<__nv_bfloat16>(ctx, p, grid, 3));
+  } else MB_FOR_ELEMENT(dtype, {
     const uintptr_t word = 4 * sizeof(T);
     const bool vec = p.dim % 4 == 0 && q_stride % 4 == 0 && kv::aligned(q, word) && kv::aligned(k_cache, word) && kv::aligned(v_cache, word);
     e = rows == 8 ? launch_cores<T, 8>(ctx, p, grid, vec) : rows == 4 ? launch_cores<T, 4>(ctx, p, grid, vec)

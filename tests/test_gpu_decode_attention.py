@@ -112,6 +112,16 @@ def test_long(ctx, name, batch, heads, kv_heads, dim, longest):
     Case(ctx, name, lengths, heads, kv_heads, dim, 32, seed=batch).run().check()
 
 
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+def test_on_cuda_cores(ctx, name):
+    """The kernel of fp32 and odd rows serves 16-bit types too ("tensor_cores" 0)."""
+    ctx.set_option("tensor_cores", 0)
+    try:
+        Case(ctx, name, [0, 1, 100, 1000], 10, 2, 128, 16, seed=3).run().check()
+    finally:
+        ctx.set_option("tensor_cores", 1)
+
+
 @pytest.mark.parametrize("name", ["f32", "bf16"])
 @pytest.mark.parametrize("window", [1, 7, 64, 500, 100000])
 def test_window(ctx, name, window):
