@@ -7,9 +7,11 @@
 // the runs are as many as fill the SMs, and the block that arrives last of a head's runs joins them.
 // Slots behind the length, outside the window or in a page that the pool lacks are -inf before the maximum, and their values
 // zeros: 0 times the NaN that an unused row may hold would be NaN.
+#include <algorithm>
 #include <cmath>
 
 #include "elements.cuh"
+#include "gemm_u8_cut.cuh"
 #include "kv_cache.h"
 #include "sm100_ptx.cuh"
 
@@ -18,6 +20,8 @@ namespace {
 constexpr int THREADS = 128;
 constexpr int WARPS = THREADS / 32;
 constexpr int MAX_SPLITS = 128;
+constexpr int LEAST_RUN = 128;   // slots that are worth a block of their own (1000 slots, 8 heads: 64 12.2 us, 128 10.8, 256 13.7)
+constexpr int SCANNED = 1024;    // sequences whose lengths every block reads
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 struct AttentionParams {
@@ -27,39 +31,144 @@ struct AttentionParams {
   float *lse;
   float *logits;        // [batch][heads][logits_stride], in powers of two; null: no weights asked for
   float *lse2;          // [batch][heads], beside them
-  float *partial;       // of (unit, run): row maxima, row sums, rows of dim
+  float *partial;       // of a run: row maxima, row sums, rows of `pitch` values
   unsigned *arrived;    // of a unit
   const float *weights_in;
   float *weights_out;
   int64_t q_stride, out_stride, num_pages, logits_stride, weights_stride, window;
-  int heads, kv_heads, group, blocks, dim, page_size, max_pages, longest, splits, split_len;
+  int batch, heads, kv_heads, group, blocks, dim, pitch, page_size, max_pages, longest, resident;
+  int cluster;                 // above 1: every head's slots over a cluster of so many blocks
+  int fixed_runs, fixed_run;   // batches above SCANNED: every head has so many runs of so many slots
   uint32_t page_mul, page_shift;
   float scale2;         // scale log2(e)
   int *status;
 };
 
-// Which part of the problem a block has.
+// Which part of the problem a block has.  The lengths are in device memory, so the blocks cut the work themselves: all slots of all
+// heads over the blocks that are resident at once give a run's length, a sequence has as many runs as it needs, and a
+// prefix sum over the sequences says whose run this block's is.  No block is without work but the few behind the last run, and a
+// batch of one long and many short sequences fills the SMs as well as one of equals.  (Runs cut by the longest sequence, which
+// the host knows: a batch of 32 from 1 to 4096 slots took 57 us instead of 51.)
 struct Place {
-  int unit, batch, kv_head, head0, heads, split, active, begin, end;
-  __device__ __forceinline__ Place(const AttentionParams &p, int rows) {
+  int unit, batch, kv_head, head0, heads, split, active, first, begin, end;   // slots from `first` on; the run is begin .. end
+  int record;                                                                 // of the unit's first run; the next ones p.blocks apart
+
+  // Slots of a sequence that a run is made of; they begin at a multiple of `chunk`, below `first` where a window does not.
+  static __device__ __forceinline__ int slots_of(const AttentionParams &p, int b, int chunk, int *first, int *from, bool *bad) {
+    const int length = kv::usable_length(mb_load(p.lengths + b), p.longest, bad);
+    *first = kv::window_begin(length, p.window);
+    *from = *first / chunk * chunk;
+    return length - *from;
+  }
+  static __device__ __forceinline__ int runs_of(const AttentionParams &p, int slots, int run) {
+    return max(1, static_cast<int>((static_cast<unsigned>(slots) + run - 1) / run));
+  }
+
+  // false: there is no such run.
+  __device__ __forceinline__ bool find(const AttentionParams &p, int rows, int chunk) {
+    __shared__ long long sums[WARPS];
+    __shared__ int counts[WARPS], found[2];
+    const int t = threadIdx.x, lane = t % 32, warp = t / 32, per_run = p.kv_heads * p.blocks;
+    int from;
+    bool bad;
+    if (p.cluster > 1) {
+      split = static_cast<int>(sm100::cluster_ctarank());
+      int x = blockIdx.x / p.cluster;
+      unit = x;
+      const int block = x % p.blocks;
+      x /= p.blocks;
+      kv_head = x % p.kv_heads;
+      batch = x / p.kv_heads;
+      const int slots = slots_of(p, batch, chunk, &first, &from, &bad);
+      if (bad && t == 0) mb_report_bad_index(p.status);
+      const int run = static_cast<int>((static_cast<unsigned>(slots) + p.cluster * 16 - 1) / (p.cluster * 16)) * 16;
+      active = p.cluster;
+      record = 0;
+      place(p, rows, block, from, slots, run);
+      if (begin > from + slots) begin = end = from + slots;
+      return true;
+    }
+    if (p.fixed_runs > 0) {
+      int x = blockIdx.x;
+      const int block = x % p.blocks;
+      x /= p.blocks;
+      split = x % p.fixed_runs;
+      unit = x / p.fixed_runs * p.blocks + block;
+      record = x / p.fixed_runs * p.fixed_runs * p.blocks + block;
+      kv_head = x / p.fixed_runs % p.kv_heads;
+      batch = x / p.fixed_runs / p.kv_heads;
+      const int slots = slots_of(p, batch, chunk, &first, &from, &bad);
+      if (bad && t == 0) mb_report_bad_index(p.status);
+      active = runs_of(p, slots, p.fixed_run);
+      if (split >= active) return false;
+      place(p, rows, block, from, slots, p.fixed_run);
+      return true;
+    }
+    long long total = 0;
+    for (int b = t; b < p.batch; b += THREADS) {
+      total += slots_of(p, b, chunk, &first, &from, &bad);
+      if (bad && blockIdx.x == 0) mb_report_bad_index(p.status);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if (lane == 0) sums[warp] = total;
+    __syncthreads();
+    total = 0;
+    for (int w = 0; w < WARPS; ++w) total += sums[w];
+    const long long share = (total * per_run + p.resident - 1) / p.resident;
+    const int run = static_cast<int>(min(max(static_cast<long long>(LEAST_RUN), (share + 63) / 64 * 64), 0x7fffffc0ll));
+    int before = 0;   // runs of the sequences in front of this round's
+    for (int base = 0; base < p.batch; base += THREADS) {
+      const int b = base + t;
+      int slots = 0, mine = 0;
+      if (b < p.batch) {
+        slots = slots_of(p, b, chunk, &first, &from, &bad);
+        mine = runs_of(p, slots, run) * per_run;
+      }
+      int upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      if (lane == 31) counts[warp] = upto;
+      __syncthreads();
+      int all = 0;
+      for (int w = 0; w < WARPS; ++w) {
+        if (w == warp) upto += all;
+        all += counts[w];
+      }
+      upto += before;
+      const int x = blockIdx.x;
+      if (x < upto && x >= upto - mine) {
+        found[0] = b;
+        found[1] = upto - mine;
+      }
+      before += all;
+      __syncthreads();
+      if (x < before) break;
+    }
+    if (static_cast<int>(blockIdx.x) >= before) return false;
+    batch = found[0];
+    const int slots = slots_of(p, batch, chunk, &first, &from, &bad);
+    active = runs_of(p, slots, run);
     // (blocks of heads that share a run follow one another, so that the run comes from memory once)
-    int x = blockIdx.x;
+    int x = blockIdx.x - found[1];
     const int block = x % p.blocks;
     x /= p.blocks;
-    split = x % p.splits;
-    x /= p.splits;
-    kv_head = x % p.kv_heads;
-    batch = x / p.kv_heads;
-    unit = x * p.blocks + block;
+    split = x % active;
+    kv_head = x / active;
+    unit = (batch * p.kv_heads + kv_head) * p.blocks + block;
+    record = found[1] + kv_head * active * p.blocks + block;
+    place(p, rows, block, from, slots, run);
+    return true;
+  }
+
+  __device__ __forceinline__ void place(const AttentionParams &p, int rows, int block, int from, int slots, int run) {
     head0 = kv_head * p.group + block * rows;
     heads = min(rows, p.group - block * rows);
-    bool bad;
-    const int length = kv::usable_length(mb_load(p.lengths + batch), p.longest, &bad);
-    if (bad && threadIdx.x == 0) mb_report_bad_index(p.status);
-    const int first = kv::window_begin(length, p.window);
-    active = max(1, (length - first + p.split_len - 1) / p.split_len);
-    begin = first + split * p.split_len;
-    end = min(begin + p.split_len, length);
+    begin = from + split * run;
+    end = from + slots - begin < run ? from + slots : begin + run;
   }
 };
 
@@ -71,17 +180,33 @@ __device__ __forceinline__ int64_t slot_offset(const AttentionParams &p, const i
   return at;
 }
 
-// What `W` warps of the block hold of their slots -- per row a maximum, a sum and `dim` values `pitch` apart -- joined, and
-// written as the result or as a run's part of it.  All in shared memory; coef: W x R floats of room, total: 2 R.
+__device__ __forceinline__ float load_remote(uint32_t addr, int rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(sm100::mapa_shared(addr, rank)) : "memory");
+  return v;
+}
+
+// The log-sum-exp of the block's row h, for the caller and for the weights.
+__device__ __forceinline__ void tell(const AttentionParams &p, const Place &at, int h, float m, float l) {
+  const int64_t to = static_cast<int64_t>(at.batch) * p.heads + at.head0 + h;
+  const float lse2 = l == 0.f ? -INFINITY : m + log2f(l);
+  if (p.lse != nullptr) p.lse[to] = lse2 * LN2;
+  if (p.logits != nullptr) p.lse2[to] = lse2;
+}
+
+// What the warps of the block hold of their slots -- per row a maximum, a sum and `dim` values `pitch` apart -- joined, and
+// written as the result or as a run's part of it.  All in shared memory; coef: WARPS x R floats of room, total: 2 R; acc is room for
+// 2 R MAX_SPLITS floats when its values have been read.
 template <typename T, int R>
-__device__ void finish(const AttentionParams &p, const Place &at, int W, int pitch, const float *top, const float *sum, const float *acc,
+__device__ void finish(const AttentionParams &p, const Place &at, int pitch, const float *top, const float *sum, float *room,
                        float *coef, float *total) {
+  const float *acc = room;
   __shared__ int last;
   const int t = threadIdx.x;
   if (t < at.heads) {
     float m = -INFINITY, l = 0.f;
-    for (int w = 0; w < W; ++w) m = fmaxf(m, top[w * R + t]);
-    for (int w = 0; w < W; ++w) {
+    for (int w = 0; w < WARPS; ++w) m = fmaxf(m, top[w * R + t]);
+    for (int w = 0; w < WARPS; ++w) {
       const float c = top[w * R + t] == -INFINITY ? 0.f : exp2f(top[w * R + t] - m);
       coef[w * R + t] = c;
       l += sum[w * R + t] * c;
@@ -90,19 +215,60 @@ __device__ void finish(const AttentionParams &p, const Place &at, int W, int pit
     total[R + t] = l;
   }
   __syncthreads();
-  const bool whole = at.active == 1;
-  float *part = whole ? nullptr : p.partial + (static_cast<int64_t>(at.unit) * p.splits + at.split) * R * (p.dim + 2);
-  for (int i = t; i < at.heads * p.dim; i += THREADS) {
-    const int h = i / p.dim, d = i - h * p.dim;
-    float o = 0.f;
-    for (int w = 0; w < W; ++w) o += acc[(w * R + h) * pitch + d] * coef[w * R + h];
-    if (whole) {
-      const float l = total[R + h];
-      static_cast<T *>(p.out)[at.batch * p.out_stride + static_cast<int64_t>(at.head0 + h) * p.dim + d] =
-          elem::narrow<T>(l == 0.f ? 0.f : o / l);
-    } else {
-      part[2 * R + h * p.dim + d] = o;
+  const bool whole = at.active == 1, apart = p.cluster > 1;   // apart: the runs of a head are the blocks of a cluster
+  constexpr int HEAD = R == 1 ? 4 : 2 * R;   // (the values behind them by 16 bytes)
+  const int record = HEAD + R * p.pitch, words = p.pitch / 4;
+  float *part = whole || apart ? nullptr : p.partial + static_cast<int64_t>(at.record + at.split * p.blocks) * record;
+  const auto store = [&](int h, int d, float4 o, float l) {
+    T *to = static_cast<T *>(p.out) + at.batch * p.out_stride + static_cast<int64_t>(at.head0 + h) * p.dim + d;
+    const float v[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (d + j < p.dim) to[j] = elem::narrow<T>(l == 0.f ? 0.f : v[j] / l);
+  };
+  for (int i = t; i < at.heads * words; i += THREADS) {
+    const int h = i / words, d = (i - h * words) * 4;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float4 v = *reinterpret_cast<const float4 *>(acc + (w * R + h) * pitch + d);
+      const float c = coef[w * R + h];
+      o.x += v.x * c;
+      o.y += v.y * c;
+      o.z += v.z * c;
+      o.w += v.w * c;
     }
+    if (whole) store(h, d, o, total[R + h]);
+    else if (apart) *reinterpret_cast<float4 *>(room + h * pitch + d) = o;   // (over the first warp's, which only this thread reads)
+    else *reinterpret_cast<float4 *>(part + HEAD + h * p.pitch + d) = o;
+  }
+  if (apart) {
+    // every block joins its share of the values out of all blocks' shared memory
+    sm100::cluster_sync_all();
+    const uint32_t tops = sm100::smem_u32(total), values = sm100::smem_u32(room);
+    for (int i = at.split * THREADS + t; i < at.heads * words; i += p.cluster * THREADS) {
+      const int h = i / words, d = (i - h * words) * 4;
+      float m = -INFINITY, l = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int s = 0; s < p.cluster; ++s) {
+        const float ms = load_remote(tops + h * 4, s), ls = load_remote(tops + (R + h) * 4, s);
+        float4 v;
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(sm100::mapa_shared(values + (h * pitch + d) * 4, s)) : "memory");
+        const float top = fmaxf(m, ms), old = m == -INFINITY ? 0.f : exp2f(m - top), c = ms == -INFINITY ? 0.f : exp2f(ms - top);
+        l = l * old + ls * c;
+        o.x = o.x * old + v.x * c;
+        o.y = o.y * old + v.y * c;
+        o.z = o.z * old + v.z * c;
+        o.w = o.w * old + v.w * c;
+        m = top;
+      }
+      store(h, d, o, l);
+      if (d == 0) tell(p, at, h, m, l);
+    }
+    sm100::cluster_sync_all();   // (no block may leave while another reads its shared memory)
+    return;
   }
   if (!whole) {
     if (t < at.heads) {
@@ -116,38 +282,59 @@ __device__ void finish(const AttentionParams &p, const Place &at, int W, int pit
     if (!last) return;
     __threadfence();
     if (t == 0) p.arrived[at.unit] = 0;
-    const float *parts = p.partial + static_cast<int64_t>(at.unit) * p.splits * R * (p.dim + 2);
-    const int64_t step = R * (p.dim + 2);
-    if (t < at.heads) {
-      float m = -INFINITY, l = 0.f;
-      for (int s = 0; s < at.active; ++s) m = fmaxf(m, __ldcg(parts + s * step + t));
-      for (int s = 0; s < at.active; ++s) {
-        const float ms = __ldcg(parts + s * step + t);
-        l += __ldcg(parts + s * step + R + t) * (ms == -INFINITY ? 0.f : exp2f(ms - m));
-      }
-      total[t] = m;
-      total[R + t] = l;
+    // all runs' maxima and sums at once, then a warp per row, then the values, four to a load and AT_ONCE runs in flight
+    constexpr int AT_ONCE = 8;
+    const float *parts = p.partial + static_cast<int64_t>(at.record) * record;
+    const int64_t step = static_cast<int64_t>(record) * p.blocks;
+    float *tops = room, *sums = room + MAX_SPLITS * R;
+    for (int i = t; i < at.active * R; i += THREADS) {
+      const int s = i / R, h = i % R;
+      const bool used = h < at.heads;
+      tops[i] = used ? __ldcg(parts + s * step + h) : -INFINITY;
+      sums[i] = used ? __ldcg(parts + s * step + R + h) : 0.f;
     }
     __syncthreads();
-    for (int i = t; i < at.heads * p.dim; i += THREADS) {
-      const int h = i / p.dim, d = i - h * p.dim;
-      const float m = total[h], l = total[R + h];
-      float o = 0.f;
-      for (int s = 0; s < at.active; ++s) {
-        const float ms = __ldcg(parts + s * step + h);
-        o += __ldcg(parts + s * step + 2 * R + i) * (ms == -INFINITY ? 0.f : exp2f(ms - m));
+    for (int h = t / 32; h < at.heads; h += WARPS) {
+      float m = -INFINITY, l = 0.f;
+      for (int s = t % 32; s < at.active; s += 32) m = fmaxf(m, tops[s * R + h]);
+#pragma unroll
+      for (int o = 16; o > 0; o /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      for (int s = t % 32; s < at.active; s += 32) {
+        const float ms = tops[s * R + h], c = ms == -INFINITY ? 0.f : exp2f(ms - m);
+        tops[s * R + h] = c;
+        l += sums[s * R + h] * c;
       }
-      static_cast<T *>(p.out)[at.batch * p.out_stride + static_cast<int64_t>(at.head0 + h) * p.dim + d] =
-          elem::narrow<T>(l == 0.f ? 0.f : o / l);
+#pragma unroll
+      for (int o = 16; o > 0; o /= 2) l += __shfl_xor_sync(0xffffffffu, l, o);
+      if (t % 32 == 0) {
+        total[h] = m;
+        total[R + h] = l;
+      }
+    }
+    __syncthreads();
+    for (int i = t; i < at.heads * words; i += THREADS) {
+      const int h = i / words, d = (i - h * words) * 4;
+      const float *from = parts + HEAD + h * p.pitch + d;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int s0 = 0; s0 < at.active; s0 += AT_ONCE) {
+        float4 v[AT_ONCE];
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j)
+          if (s0 + j < at.active) v[j] = __ldcg(reinterpret_cast<const float4 *>(from + (s0 + j) * step));
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j)
+          if (s0 + j < at.active) {
+            const float c = tops[(s0 + j) * R + h];
+            o.x += v[j].x * c;
+            o.y += v[j].y * c;
+            o.z += v[j].z * c;
+            o.w += v[j].w * c;
+          }
+      }
+      store(h, d, o, total[R + h]);
     }
   }
-  if (t < at.heads) {
-    const float m = total[t], l = total[R + t];
-    const int64_t to = static_cast<int64_t>(at.batch) * p.heads + at.head0 + t;
-    const float lse2 = l == 0.f ? -INFINITY : m + log2f(l);
-    if (p.lse != nullptr) p.lse[to] = lse2 * LN2;
-    if (p.logits != nullptr) p.lse2[to] = lse2;
-  }
+  if (t < at.heads) tell(p, at, t, total[t], total[R + t]);
 }
 
 // ---- on CUDA cores: every type, size and alignment -----------------------------------------------------------------------
@@ -177,11 +364,11 @@ __global__ void __launch_bounds__(THREADS) paged_attention_kernel(const Attentio
   __shared__ float scores[WARPS][SLOTS * R], fix[WARPS][R];
   __shared__ int64_t rows[WARPS][SLOTS];
   __shared__ float top_s[WARPS * R], sum_s[WARPS * R], coef[WARPS * R], total[2 * R];
-  __shared__ float acc_s[WARPS * R * DIM];
+  __shared__ __align__(16) float acc_s[WARPS * R * DIM < 2 * R * MAX_SPLITS ? 2 * R * MAX_SPLITS : WARPS * R * DIM];
   mb_grid_dep_launch();
   mb_grid_dep_wait();
-  const Place at(p, R);
-  if (at.split >= at.active) return;
+  Place at;
+  if (!at.find(p, R, 1)) return;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int mine = lane / LANES, word = lane % LANES;   // which slot of a pass, which words of its row
   const T *q = static_cast<const T *>(p.q), *k = static_cast<const T *>(p.k), *v = static_cast<const T *>(p.v);
@@ -315,16 +502,18 @@ __global__ void __launch_bounds__(THREADS) paged_attention_kernel(const Attentio
     }
   }
   __syncthreads();
-  finish<T, R>(p, at, WARPS, DIM, top_s, sum_s, acc_s, coef, total);
+  finish<T, R>(p, at, DIM, top_s, sum_s, acc_s, coef, total);
 }
 
 // ---- on the tensor cores: 16-bit types, rows of whole 16-byte words -----------------------------------------------------------
 //
-// Up to 16 query heads are the rows of mma.sync m16n8k16 (a decode step has no 128 rows for tcgen05 to multiply, and the cache's bytes
-// bound it by far: 16 rows cost 16 operations a byte where 250 would be needed).  Every warp has a ring of its own in shared
-// memory that its cp.asyncs fill with CHUNK slots' keys and values at a time, two stages ahead, so that no barrier joins warps
-// before the end.  Rows are swizzled in 16-byte words for ldmatrix.  Probabilities are multiplied as two 16-bit values, hi + lo:
-// their sum is the fp32 one to 2^-16 (bf16) or 2^-22, and the second product costs nothing that the memory does not hide.
+// mma.sync m16n8k16 with slots as rows and 8 query heads as columns: S^T = K Q^T, then O^T = V^T P^T.  (A decode step has no 128 rows
+// for tcgen05 to multiply, and the cache's bytes bound it by far.  With heads as the 16 rows, as a prompt's attention has
+// them, a group of four or eight leaves half of every product and of every exponential unused: 787 instructions per 16 slots where this
+// form takes about 200, and 210 us instead of 165 for two sequences of 120001.)  Every warp has a ring of its own in shared memory that
+// its cp.asyncs fill with CHUNK slots' keys and values at a time, so that no barrier joins warps before the end.  Rows are
+// swizzled in 16-byte words for ldmatrix.  Probabilities are multiplied as two 16-bit values, hi + lo: their sum is the fp32 one to
+// 2^-16 (bf16) or 2^-22, and the second product costs nothing that the memory does not hide.
 
 template <typename T> struct Mma;
 template <> struct Mma<__half> {
@@ -364,75 +553,88 @@ __device__ __forceinline__ void load_matrices(uint32_t addr, uint32_t (&r)[4]) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 
+// An 8 x 8 matrix of 16-bit values, two of a row to a lane, transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+__device__ __forceinline__ void copy_word(uint32_t dst, const void *src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_word(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
 template <int DIM>
 struct Ring {
-  static constexpr int CHUNK = DIM == 64 ? 32 : 16;         // slots
-  static constexpr int ROW = DIM * 2, WORDS = DIM / 8;      // bytes of a row, its 16-byte words
+  static constexpr int CHUNK = 16;                            // slots
+  static constexpr int ROW = DIM * 2, WORDS = DIM / 8;        // bytes of a row, its 16-byte words
   static constexpr int PART = CHUNK * ROW, STAGE = 2 * PART;  // keys, then values
-  static constexpr int STAGES = 3;
+  static constexpr int STAGES = DIM == 128 ? 2 : 3;
   static constexpr int BYTES = WARPS * STAGES * STAGE;
-  static constexpr int PITCH = DIM + 4;                     // floats between rows of the accumulators at the end
+  static constexpr int PITCH = DIM + 4;                       // floats between rows of the accumulators at the end
+  static_assert(2 * 16 * MAX_SPLITS * 4 <= BYTES, "what joins the runs reuses it too");
   static_assert(WARPS * 16 * PITCH * 4 <= BYTES, "accumulators reuse the ring");
 };
 
-template <typename T, int DIM>
+// HEADS: tiles of 8 query heads.  WHOLE: a chunk of slots lies in one page, and rows have DIM values.
+template <typename T, int DIM, int HEADS, bool WHOLE>
 __global__ void __launch_bounds__(THREADS) paged_attention_mma_kernel(const AttentionParams p) {
   using G = Ring<DIM>;
-  constexpr int R = 16, CHUNK = G::CHUNK, KEY_TILES = CHUNK / 8, DIM_STEPS = DIM / 16, STAGES = G::STAGES;
+  constexpr int R = 8 * HEADS, CHUNK = G::CHUNK, DIM_STEPS = DIM / 16, STAGES = G::STAGES;
   extern __shared__ __align__(1024) uint8_t ring[];
   __shared__ unsigned valid[WARPS][STAGES];
   __shared__ float top_s[WARPS * R], sum_s[WARPS * R], coef[WARPS * R], total[2 * R];
   mb_grid_dep_launch();
   mb_grid_dep_wait();
-  const Place at(p, R);
-  if (at.split >= at.active) return;
+  Place at;
+  if (!at.find(p, R, CHUNK)) return;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = lane / 4, pair = lane % 4;
   const T *k = static_cast<const T *>(p.k), *v = static_cast<const T *>(p.v);
   const int32_t *table = p.table + static_cast<int64_t>(at.batch) * p.max_pages;
   const uint32_t mine = sm100::smem_u32(ring) + warp * STAGES * G::STAGE;
 
-  // the queries of rows `row` and `row` + 8
-  uint32_t q[DIM_STEPS][4];
-#pragma unroll
-  for (int s = 0; s < DIM_STEPS; ++s)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int h = row + i % 2 * 8, d = s * 16 + i / 2 * 8 + pair * 2;
-      elem::Vec<T, 2> two;
-      two.word = 0;
-      if (h < at.heads && d < p.dim) {
-        const T *src = static_cast<const T *>(p.q) + at.batch * p.q_stride + static_cast<int64_t>(at.head0 + h) * p.dim + d;
-        two.v[0] = mb_load(src);
-        two.v[1] = mb_load(src + 1);
-      }
-      q[s][i] = two.word;
-    }
-  float acc[2 * DIM_STEPS][4], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < 2 * DIM_STEPS; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-
   const int chunks = (at.end - at.begin + CHUNK - 1) / CHUNK;   // of all warps; this one has warp, warp + WARPS, ..
-  const auto offset_of = [&](int chunk) -> int64_t {
+  // Where chunk's slot l lies, for lane l; with WHOLE, where its first slot does, if all of them are there, else -1.
+  const auto slot_of = [&](int chunk) -> int64_t {
     const int slot = at.begin + chunk * CHUNK + lane;
-    return lane < CHUNK && chunk < chunks && slot < at.end ? slot_offset(p, table, at.kv_head, slot) : -1;
+    return lane < CHUNK && slot >= at.first && slot < at.end ? slot_offset(p, table, at.kv_head, slot) : -1;
   };
-  // `where`: lane l's offset of the chunk's slot l
+  const auto offset_of = [&](int chunk) -> int64_t {
+    if (chunk >= chunks) return -1;
+    if (!WHOLE) return slot_of(chunk);
+    const int slot = at.begin + chunk * CHUNK;
+    return slot >= at.first && slot + CHUNK <= at.end ? slot_offset(p, table, at.kv_head, slot) : -1;
+  };
+  const int word = lane % G::WORDS, line = lane / G::WORDS;
+  constexpr int LINES = 32 / G::WORDS;   // rows that one instruction copies
   const auto fetch = [&](int chunk, int stage, int64_t where) {
     if (chunk < chunks) {
-      const unsigned ok = __ballot_sync(0xffffffffu, where >= 0);
-      if (lane == 0) valid[warp][stage] = ok;
-      const int word = lane % G::WORDS;
+      const uint32_t to = mine + stage * G::STAGE + line * G::ROW;
+      if (WHOLE && where >= 0) {
+        const T *ks = k + where + line * DIM + word * 8, *vs = v + where + line * DIM + word * 8;
+        if (lane == 0) valid[warp][stage] = 0xffffu;
 #pragma unroll
-      for (int i = 0; i < CHUNK * G::WORDS / 32; ++i) {
-        const int r = i * (32 / G::WORDS) + lane / G::WORDS;
-        const int64_t from = __shfl_sync(0xffffffffu, where, r);
-        const bool there = from >= 0 && word * 8 < p.dim;
-        const int64_t src = there ? from + word * 8 : 0;
-        const uint32_t dst = mine + stage * G::STAGE + r * G::ROW + ((word ^ (r & 7)) << 4);
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(k + src), "r"(there ? 16 : 0) : "memory");
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + G::PART), "l"(v + src), "r"(there ? 16 : 0) : "memory");
+        for (int i = 0; i < CHUNK / LINES; ++i) {
+          const uint32_t dst = to + i * LINES * G::ROW + ((word ^ ((i * LINES + line) & 7)) << 4);
+          copy_word(dst, ks + i * LINES * DIM);
+          copy_word(dst + G::PART, vs + i * LINES * DIM);
+        }
+      } else {
+        if (WHOLE) where = slot_of(chunk);
+        const unsigned ok = __ballot_sync(0xffffffffu, where >= 0);
+        if (lane == 0) valid[warp][stage] = ok;
+#pragma unroll
+        for (int i = 0; i < CHUNK / LINES; ++i) {
+          const int64_t from = __shfl_sync(0xffffffffu, where, i * LINES + line);
+          const bool there = from >= 0 && word * 8 < p.dim;
+          const int64_t src = there ? from + word * 8 : 0;
+          const uint32_t dst = to + i * LINES * G::ROW + ((word ^ ((i * LINES + line) & 7)) << 4);
+          copy_word(dst, k + src, there ? 16 : 0);
+          copy_word(dst + G::PART, v + src, there ? 16 : 0);
+        }
       }
     }
     sm100::cp_async_commit();
@@ -440,6 +642,44 @@ __global__ void __launch_bounds__(THREADS) paged_attention_mma_kernel(const Atte
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) fetch(warp + s * WARPS, s, offset_of(warp + s * WARPS));
   int64_t ahead = offset_of(warp + (STAGES - 1) * WARPS);
+
+  // the queries: head `row` of each tile
+  uint32_t q[HEADS][DIM_STEPS][2];
+#pragma unroll
+  for (int t = 0; t < HEADS; ++t)
+#pragma unroll
+    for (int s = 0; s < DIM_STEPS; ++s)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int h = t * 8 + row, d = s * 16 + i * 8 + pair * 2;
+        elem::Vec<T, 2> two;
+        two.word = 0;
+        if (h < at.heads && d < p.dim) {
+          const T *src = static_cast<const T *>(p.q) + at.batch * p.q_stride + static_cast<int64_t>(at.head0 + h) * p.dim + d;
+          two.v[0] = mb_load(src);
+          two.v[1] = mb_load(src + 1);
+        }
+        q[t][s][i] = two.word;
+      }
+  // heads 2 pair and 2 pair + 1 of each tile: values row and row + 8 of every 16, maximum, and this lane's part of the sum
+  float acc[HEADS][DIM_STEPS][4], top[HEADS][2], sum[HEADS][2];
+#pragma unroll
+  for (int t = 0; t < HEADS; ++t) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) top[t][j] = -INFINITY, sum[t][j] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DIM_STEPS; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[t][d][j] = 0.f;
+  }
+  // ldmatrix: keys row lane % 16, values row lane % 8 + lane / 16 * 8; their words' swizzle within 128 bytes
+  const uint32_t key_row = lane % 16 * G::ROW, value_row = (lane % 8 + lane / 16 * 8) * G::ROW;
+  uint32_t key_word[4], value_word[4];
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    key_word[d] = key_row + (((2 * d + lane / 16) ^ (lane & 7)) << 4);
+    value_word[d] = value_row + (((2 * d + lane / 8 % 2) ^ (lane & 7)) << 4);
+  }
 
   int stage = 0;
   for (int chunk = warp; chunk < chunks; chunk += WARPS) {
@@ -449,81 +689,91 @@ __global__ void __launch_bounds__(THREADS) paged_attention_mma_kernel(const Atte
     ahead = offset_of(chunk + STAGES * WARPS);
     const uint32_t keys = mine + stage * G::STAGE, values = keys + G::PART;
     const unsigned ok = valid[warp][stage];
-    float s[KEY_TILES][4];
+    // slots row and row + 8: s[t][0, 1] and s[t][2, 3] are heads 2 pair and 2 pair + 1
+    float s[HEADS][4];
 #pragma unroll
-    for (int t = 0; t < KEY_TILES; ++t)
+    for (int t = 0; t < HEADS; ++t)
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[t][j] = 0.f;
 #pragma unroll
-    for (int d = 0; d < DIM_STEPS; ++d)
+    for (int d = 0; d < DIM_STEPS; ++d) {
+      uint32_t a[4];
+      load_matrices<false>(keys + key_word[d % 4] + d / 4 * 128, a);
 #pragma unroll
-      for (int t = 0; t < KEY_TILES; t += 2) {
-        uint32_t b[4];
-        const int r = t * 8 + lane % 8 + lane / 16 * 8, word = 2 * d + lane / 8 % 2;
-        load_matrices<false>(keys + r * G::ROW + ((word ^ (r & 7)) << 4), b);
-        Mma<T>::run(s[t], q[d], b[0], b[1]);
-        Mma<T>::run(s[t + 1], q[d], b[2], b[3]);
-      }
-    const int slot = at.begin + chunk * CHUNK + pair * 2;
-    float m[2] = {top[0], top[1]};
+      for (int t = 0; t < HEADS; ++t) Mma<T>::run(s[t], a, q[t][d][0], q[t][d][1]);
+    }
 #pragma unroll
-    for (int t = 0; t < KEY_TILES; ++t)
+    for (int t = 0; t < HEADS; ++t)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[t][j] = (ok >> (t * 8 + pair * 2 + j % 2) & 1u) != 0 ? s[t][j] * p.scale2 : -INFINITY;
-        m[j / 2] = fmaxf(m[j / 2], s[t][j]);
-      }
+      for (int j = 0; j < 4; ++j) s[t][j] *= p.scale2;
+    if (ok != 0xffffu) {
+#pragma unroll
+      for (int t = 0; t < HEADS; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if ((ok >> (row + j / 2 * 8) & 1u) == 0) s[t][j] = -INFINITY;
+    }
     if (p.logits != nullptr) {
+      const int slot = at.begin + chunk * CHUNK + row;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (row + 8 * h < at.heads) {
-          float *to = p.logits + (static_cast<int64_t>(at.batch) * p.heads + at.head0 + row + 8 * h) * p.logits_stride + slot;
+      for (int t = 0; t < HEADS; ++t)
 #pragma unroll
-          for (int t = 0; t < KEY_TILES; ++t)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              if (slot + t * 8 + j < at.end) to[t * 8 + j] = s[t][2 * h + j];
+        for (int j = 0; j < 4; ++j) {
+          const int h = t * 8 + pair * 2 + j % 2, n = slot + j / 2 * 8;
+          if (h < at.heads && n < at.end)
+            p.logits[(static_cast<int64_t>(at.batch) * p.heads + at.head0 + h) * p.logits_stride + n] = s[t][j];
         }
     }
+    float m[HEADS][2];
     bool grew = false;
-    float back[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      m[h] = fmaxf(m[h], __shfl_xor_sync(0xffffffffu, m[h], 1));
-      m[h] = fmaxf(m[h], __shfl_xor_sync(0xffffffffu, m[h], 2));
-      grew = grew || m[h] != top[h];
-      const float safe = m[h] == -INFINITY ? 0.f : m[h];
-      back[h] = exp2f(top[h] - safe);
-      top[h] = m[h];
-      m[h] = safe;
-      sum[h] *= back[h];
-    }
+    for (int t = 0; t < HEADS; ++t)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        m[t][j] = fmaxf(s[t][j], s[t][j + 2]);
+        grew = grew || m[t][j] > top[t][j];
+      }
+    // (a maximum that no lane exceeds stays: neither the exchange nor the factors are needed)
     if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-      for (int i = 0; i < 2 * DIM_STEPS; ++i)
+      for (int t = 0; t < HEADS; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] *= back[j / 2];
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int o = 4; o < 32; o *= 2) m[t][j] = fmaxf(m[t][j], __shfl_xor_sync(0xffffffffu, m[t][j], o));
+          m[t][j] = fmaxf(m[t][j], top[t][j]);
+          const float back = m[t][j] == -INFINITY ? 1.f : exp2f(top[t][j] - m[t][j]);
+          top[t][j] = m[t][j];
+          sum[t][j] *= back;
+#pragma unroll
+          for (int d = 0; d < DIM_STEPS; ++d) {
+            acc[t][d][j] *= back;
+            acc[t][d][j + 2] *= back;
+          }
+        }
+    }
+    uint32_t hi[HEADS][2], lo[HEADS][2];
+#pragma unroll
+    for (int t = 0; t < HEADS; ++t) {
+      const float m0 = top[t][0] == -INFINITY ? 0.f : top[t][0], m1 = top[t][1] == -INFINITY ? 0.f : top[t][1];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float x = exp2f(s[t][2 * i] - m0), y = exp2f(s[t][2 * i + 1] - m1);
+        sum[t][0] += x;
+        sum[t][1] += y;
+        Mma<T>::split(x, y, hi[t][i], lo[t][i]);
+        hi[t][i] = transposed(hi[t][i]);
+        lo[t][i] = transposed(lo[t][i]);
+      }
     }
 #pragma unroll
-    for (int t = 0; t < KEY_TILES; t += 2) {
-      uint32_t hi[4], lo[4];
+    for (int d = 0; d < DIM_STEPS; ++d) {
+      uint32_t a[4];
+      load_matrices<true>(values + value_word[d % 4] + d / 4 * 128, a);
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float x = exp2f(s[t + u][2 * h] - m[h]), y = exp2f(s[t + u][2 * h + 1] - m[h]);
-          sum[h] += x + y;
-          Mma<T>::split(x, y, hi[2 * u + h], lo[2 * u + h]);
-        }
-#pragma unroll
-      for (int d = 0; d < DIM_STEPS; ++d) {
-        uint32_t b[4];
-        const int r = t * 8 + lane % 16, word = 2 * d + lane / 16;
-        load_matrices<true>(values + r * G::ROW + ((word ^ (r & 7)) << 4), b);
-        Mma<T>::run(acc[2 * d], hi, b[0], b[1]);
-        Mma<T>::run(acc[2 * d + 1], hi, b[2], b[3]);
-        Mma<T>::run(acc[2 * d], lo, b[0], b[1]);
-        Mma<T>::run(acc[2 * d + 1], lo, b[2], b[3]);
+      for (int t = 0; t < HEADS; ++t) {
+        Mma<T>::run(acc[t][d], a, hi[t][0], hi[t][1]);
+        Mma<T>::run(acc[t][d], a, lo[t][0], lo[t][1]);
       }
     }
     stage = stage + 1 == STAGES ? 0 : stage + 1;
@@ -532,67 +782,97 @@ __global__ void __launch_bounds__(THREADS) paged_attention_mma_kernel(const Atte
   __syncthreads();
   float *acc_s = reinterpret_cast<float *>(ring);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
-    sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
-    if (row + 8 * h < at.heads) {
-      const int r = warp * R + row + 8 * h;
-      if (pair == 0) {
-        top_s[r] = top[h];
-        sum_s[r] = sum[h];
-      }
+  for (int t = 0; t < HEADS; ++t)
 #pragma unroll
-      for (int i = 0; i < 2 * DIM_STEPS; ++i)
-        *reinterpret_cast<float2 *>(acc_s + r * G::PITCH + i * 8 + pair * 2) = make_float2(acc[i][2 * h], acc[i][2 * h + 1]);
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int o = 4; o < 32; o *= 2) sum[t][j] += __shfl_xor_sync(0xffffffffu, sum[t][j], o);
+      const int h = t * 8 + pair * 2 + j;
+      if (h < at.heads) {
+        const int r = warp * R + h;
+        if (row == 0) {
+          top_s[r] = top[t][j];
+          sum_s[r] = sum[t][j];
+        }
+#pragma unroll
+        for (int d = 0; d < DIM_STEPS; ++d) {
+          acc_s[r * G::PITCH + d * 16 + row] = acc[t][d][j];
+          acc_s[r * G::PITCH + d * 16 + row + 8] = acc[t][d][j + 2];
+        }
+      }
     }
-  }
   __syncthreads();
-  finish<T, R>(p, at, WARPS, G::PITCH, top_s, sum_s, acc_s, coef, total);
+  finish<T, R>(p, at, G::PITCH, top_s, sum_s, acc_s, coef, total);
 }
 
-template <typename T, int DIM>
+template <typename T, int DIM, int HEADS, bool WHOLE>
 int launch_mma(mb_context *ctx, const AttentionParams &p, unsigned grid, int index) {
-  const auto kern = paged_attention_mma_kernel<T, DIM>;
+  const auto kern = paged_attention_mma_kernel<T, DIM, HEADS, WHOLE>;
+  index += (HEADS - 1) * 2 + WHOLE;
   if (!(ctx->attention_attr_mask & (1u << index))) {
     MB_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<DIM>::BYTES));
+    MB_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));   // clusters of 16
     ctx->attention_attr_mask |= 1u << index;
   }
-  MB_CUDA(ctx, mb_launch_chained(ctx, kern, dim3(grid), dim3(THREADS), Ring<DIM>::BYTES, p));
+  MB_CUDA(ctx, mb_launch_clusters(ctx, kern, grid, THREADS, Ring<DIM>::BYTES, p.cluster, p));
   return MB_SUCCESS;
 }
 
-template <typename T>
-int launch_mma(mb_context *ctx, const AttentionParams &p, unsigned grid, int index) {
-  if (p.dim <= 64) return launch_mma<T, 64>(ctx, p, grid, index);
-  if (p.dim <= 128) return launch_mma<T, 128>(ctx, p, grid, index + 1);
-  return launch_mma<T, 256>(ctx, p, grid, index + 2);
+template <typename T, int DIM>
+int launch_mma(mb_context *ctx, const AttentionParams &p, unsigned grid, int rows, int index) {
+  const bool whole = p.dim == DIM && p.page_size % Ring<DIM>::CHUNK == 0;
+  if (rows > 8) return whole ? launch_mma<T, DIM, 2, true>(ctx, p, grid, index) : launch_mma<T, DIM, 2, false>(ctx, p, grid, index);
+  return whole ? launch_mma<T, DIM, 1, true>(ctx, p, grid, index) : launch_mma<T, DIM, 1, false>(ctx, p, grid, index);
 }
 
-// What each slot has received of the query heads' probabilities, on top of what it had.
+template <typename T>
+int launch_mma(mb_context *ctx, const AttentionParams &p, unsigned grid, int rows, int index) {
+  if (p.dim <= 64) return launch_mma<T, 64>(ctx, p, grid, rows, index);
+  if (p.dim <= 128) return launch_mma<T, 128>(ctx, p, grid, rows, index + 4);
+  return launch_mma<T, 256>(ctx, p, grid, rows, index + 8);
+}
+
+// What each slot has received of the query heads' probabilities, on top of what it had.  Four slots a thread: a word of every head's
+// logits, all in flight together.
+constexpr int WEIGHT_SLOTS = 1024;   // of a block
+
 __global__ void __launch_bounds__(256) attention_weights_kernel(const AttentionParams p, int chunks) {
   mb_grid_dep_launch();
   mb_grid_dep_wait();
   const int unit = blockIdx.x / chunks, batch = unit / p.kv_heads, kv_head = unit % p.kv_heads;
-  const int slot = (blockIdx.x % chunks) * 256 + threadIdx.x;
+  const int slot = (blockIdx.x % chunks) * WEIGHT_SLOTS + threadIdx.x * 4;
   bool bad;
   const int length = kv::usable_length(mb_load(p.lengths + batch), p.longest, &bad);
   if (slot >= length) return;
+  const int first = kv::window_begin(length, p.window);
   const int64_t to = static_cast<int64_t>(unit) * p.weights_stride + slot;
-  float w = 0.f;
-  if (slot >= kv::window_begin(length, p.window)) {
+  float w[4] = {0.f, 0.f, 0.f, 0.f}, had[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) had[j] = p.weights_in != nullptr && slot + j < length ? mb_load(p.weights_in + to + j) : 0.f;
+  if (slot + 3 >= first) {
+    // (rows of logits are whole words; what is outside first .. length is not used)
     const int64_t head = static_cast<int64_t>(batch) * p.heads + kv_head * p.group;
+#pragma unroll 4
     for (int g = 0; g < p.group; ++g) {
       const float lse2 = mb_load(p.lse2 + head + g);
-      if (lse2 != -INFINITY) w += exp2f(mb_load(p.logits + (head + g) * p.logits_stride + slot) - lse2);
+      const float4 s = mb_load(reinterpret_cast<const float4 *>(p.logits + (head + g) * p.logits_stride + slot));
+      if (lse2 != -INFINITY) {
+        w[0] += exp2f(s.x - lse2);
+        w[1] += exp2f(s.y - lse2);
+        w[2] += exp2f(s.z - lse2);
+        w[3] += exp2f(s.w - lse2);
+      }
     }
   }
-  p.weights_out[to] = (p.weights_in != nullptr ? mb_load(p.weights_in + to) : 0.f) + w;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (slot + j < length) p.weights_out[to + j] = had[j] + (slot + j >= first ? w[j] : 0.f);
 }
 
 template <typename T, int R, int LANES, int N>
 cudaError_t launch_cores(mb_context *ctx, const AttentionParams &p, unsigned grid, bool vec) {
-  if (vec) return mb_launch_chained(ctx, paged_attention_kernel<T, R, LANES, N, true>, dim3(grid), dim3(THREADS), 0, p);
-  return mb_launch_chained(ctx, paged_attention_kernel<T, R, LANES, N, false>, dim3(grid), dim3(THREADS), 0, p);
+  if (vec) return mb_launch_clusters(ctx, paged_attention_kernel<T, R, LANES, N, true>, grid, THREADS, 0, p.cluster, p);
+  return mb_launch_clusters(ctx, paged_attention_kernel<T, R, LANES, N, false>, grid, THREADS, 0, p.cluster, p);
 }
 
 template <typename T, int R>
@@ -601,14 +881,6 @@ cudaError_t launch_cores(mb_context *ctx, const AttentionParams &p, unsigned gri
   if (p.dim <= 64) return launch_cores<T, R, 16, 1>(ctx, p, grid, vec);
   if (p.dim <= 128) return launch_cores<T, R, 32, 1>(ctx, p, grid, vec);
   return launch_cores<T, R, 32, 2>(ctx, p, grid, vec);
-}
-
-// The runs a head's slots are cut into: about four blocks per SM where the sequences are as long as they may be, of 64 slots at least.
-void cut_runs(const mb_context *ctx, AttentionParams &p, int64_t units) {
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(4ll * ctx->num_sms / std::max<int64_t>(units, 1), MAX_SPLITS));
-  const int64_t most = std::max<int64_t>(p.longest, 1);
-  p.split_len = static_cast<int>(std::max<int64_t>(64, ceil_div64(ceil_div64(most, want), 64) * 64));
-  p.splits = static_cast<int>(ceil_div64(most, p.split_len));
 }
 
 }  // namespace
@@ -637,12 +909,35 @@ extern "C" int mb_paged_attention(mb_context *ctx, const void *q, const void *k_
   p.status = ctx->dev_status;
 
   const bool by_mma = dtype != MB_F32 && ctx->use_tensor_cores && head_dim % 8 == 0 && kv::aligned(k_cache, 16) && kv::aligned(v_cache, 16);
-  const int rows = by_mma ? 16 : p.group >= 5 ? 8 : p.group >= 3 ? 4 : p.group;
+  const int rows = by_mma ? (p.group > 8 ? 16 : 8) : p.group >= 5 ? 8 : p.group >= 3 ? 4 : p.group;
   p.blocks = (p.group + rows - 1) / rows;
+  p.batch = static_cast<int>(batch);
+  p.pitch = static_cast<int>(align_up(p.dim, 4));
+  // As many runs as blocks are resident, and one more for each head of a sequence, whose last run is not a whole one; a sequence of one
+  // run is all that short ones have.
   const int64_t units = batch * kv_heads * p.blocks;
-  cut_runs(ctx, p, units);
-  if (units * p.splits > kv::MOST) return mb_fail(ctx, MB_UNSUPPORTED, "mb_paged_attention: too many sequences and heads");
-  const size_t partial = p.splits > 1 ? align_up(sizeof(float) * units * p.splits * rows * (p.dim + 2), 256) : 0;
+  // Work that is over before its blocks' parts could meet in memory: each head's slots over a cluster, 128 of them a block at least
+  // (1000 slots, 8 heads: 10.4 us with the runs joined by the last block, 7.7 on clusters of 8; 8192: 18.6 and 16.1 on 16).
+  constexpr int64_t SMALL = 64ll << 20;
+  const int most = by_mma ? 16 : 8;
+  p.cluster = 1;
+  if (units * p.longest * 2 * head_dim * kv::type_bytes(dtype) <= SMALL)
+    while (p.cluster < most && units * p.cluster * 2 <= 2 * ctx->num_sms && p.longest > LEAST_RUN * p.cluster) p.cluster *= 2;
+  const int per_sm = !by_mma ? (rows * p.dim >= 1024 ? 3 : 5) : p.dim > 128 ? 1 : 3;
+  const int64_t slots = per_sm * ctx->num_sms;
+  // one round of blocks where the heads leave it room, else several, so that the last one is a small part
+  p.resident = static_cast<int>(std::min<int64_t>(units * 2 <= slots ? slots - units : 4 * slots, MAX_SPLITS * kv_heads * p.blocks));
+  int64_t runs = std::min<int64_t>(units + p.resident, units * std::max<int64_t>(1, ceil_div64(p.longest + 15, LEAST_RUN)));
+  if (p.cluster > 1) {
+    runs = units * p.cluster;
+  } else if (batch > SCANNED) {
+    // (reading thousands of lengths in every block costs more than it evens out)
+    p.fixed_runs = static_cast<int>(std::min<int64_t>(16, std::max<int64_t>(1, ceil_div64(p.longest, 4096))));
+    p.fixed_run = static_cast<int>(ceil_div64(ceil_div64(std::max<int64_t>(p.longest + 15, 1), p.fixed_runs), 64) * 64);
+    runs = units * p.fixed_runs;
+  }
+  if (runs > kv::MOST) return mb_fail(ctx, MB_UNSUPPORTED, "mb_paged_attention: too many sequences and heads");
+  const size_t partial = runs > units && p.cluster == 1 ? align_up(sizeof(float) * runs * (rows * p.pitch + std::max(4, 2 * rows)), 256) : 0;
   size_t logits = 0, lse2 = 0;
   if (weights_out != nullptr && p.longest > 0) {
     p.logits_stride = align_up(p.longest, 4);
@@ -663,11 +958,11 @@ extern "C" int mb_paged_attention(mb_context *ctx, const void *q, const void *k_
     p.lse2 = reinterpret_cast<float *>(room + partial);
     p.logits = reinterpret_cast<float *>(room + partial + lse2);
   }
-  const unsigned grid = static_cast<unsigned>(units * p.splits);
+  const unsigned grid = static_cast<unsigned>(runs);
   cudaError_t e = cudaSuccess;
   if (by_mma) {
-    if (dtype == MB_F16) MB_RETURN_IF_ERROR(launch_mma<__half>(ctx, p, grid, 0));
-    else MB_RETURN_IF_ERROR(launch_mma<__nv_bfloat16>(ctx, p, grid, 3));
+    if (dtype == MB_F16) MB_RETURN_IF_ERROR(launch_mma<__half>(ctx, p, grid, rows, 0));
+    else MB_RETURN_IF_ERROR(launch_mma<__nv_bfloat16>(ctx, p, grid, rows, 12));
   } else MB_FOR_ELEMENT(dtype, {
     const uintptr_t word = 4 * sizeof(T);
     const bool vec = p.dim % 4 == 0 && q_stride % 4 == 0 && kv::aligned(q, word) && kv::aligned(k_cache, word) && kv::aligned(v_cache, word);
@@ -677,7 +972,7 @@ extern "C" int mb_paged_attention(mb_context *ctx, const void *q, const void *k_
   MB_CUDA(ctx, e);
   ctx->launches++;
   if (logits > 0) {
-    const int chunks = (p.longest + 255) / 256;
+    const int chunks = (p.longest + WEIGHT_SLOTS - 1) / WEIGHT_SLOTS;
     if (batch * kv_heads * chunks > kv::MOST) return mb_fail(ctx, MB_UNSUPPORTED, "mb_paged_attention: too many slots");
     MB_CUDA(ctx, mb_launch_chained(ctx, attention_weights_kernel, dim3(static_cast<unsigned>(batch * kv_heads * chunks)), dim3(256), 0, p, chunks));
     ctx->launches++;

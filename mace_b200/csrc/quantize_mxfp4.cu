@@ -3,6 +3,8 @@
 // A thread has eight values, so four neighbouring lanes have a block: its largest magnitude is two shuffles away, and its exponent
 // field is the scale.  Dividing by a power of two is exact, and the conversion rounds to nearest even and saturates, so the result is
 // the definition's bit for bit.
+#include <algorithm>
+
 #include "elements.cuh"
 #include "mxfp4.h"
 
@@ -19,7 +21,8 @@ struct MxParams {
   int cols, tiles;       // tiles of scales in a row of tiles
   int chunks;            // groups of EACH values in a row's tiles
   int vec;               // words of 16 bytes (fp32: two of them) are aligned
-  uint32_t chunk_mul, chunk_shift;
+  int block_rows, row_blocks;   // a block has whole rows, or a row whole blocks
+  uint32_t chunk_mul, chunk_shift, row_mul, row_shift;
 };
 
 template <typename T>
@@ -46,15 +49,30 @@ __device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
   return r;
 }
 
+// A thread's row and group of eight: with the whole tiles' groups of a row below THREADS a block has several rows, else a row
+// several blocks.  chunk may lie behind the row's last.
+__device__ __forceinline__ void place(const MxParams &p, int64_t *row, int *chunk) {
+  if (p.row_blocks == 1) {
+    const int r = static_cast<int>(fast_div(threadIdx.x, p.chunk_mul, p.chunk_shift));
+    *row = static_cast<int64_t>(blockIdx.x) * p.block_rows + r;
+    *chunk = r < p.block_rows ? static_cast<int>(threadIdx.x) - r * p.chunks : p.chunks;
+  } else {
+    const int r = static_cast<int>(fast_div(blockIdx.x, p.row_mul, p.row_shift));
+    *row = r;
+    *chunk = (static_cast<int>(blockIdx.x) - r * p.row_blocks) * THREADS + threadIdx.x;
+  }
+}
+
 // Items are (row, group of eight) of the whole tiles: a lane whose block does not exist writes the tile's zeros.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) quantize_mxfp4_kernel(const MxParams p) {
   mb_grid_dep_launch();
   mb_grid_dep_wait();
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
-  const int64_t row = item / p.chunks;
-  const int chunk = static_cast<int>(item - row * p.chunks);
-  if (row >= mx::tile_rows(p.rows) * mx::TILE_ROWS) return;   // (blocks and so groups of four lanes go together)
+  int64_t row;
+  int chunk;
+  place(p, &row, &chunk);
+  // (rows are whole groups of sixteen lanes, whose words of four scales leave together)
+  if (chunk >= p.chunks || row >= mx::tile_rows(p.rows) * mx::TILE_ROWS) return;
   const int col = chunk * EACH;
   const bool there = row < p.rows;
   float v[EACH];
@@ -80,16 +98,21 @@ __global__ void __launch_bounds__(THREADS) quantize_mxfp4_kernel(const MxParams 
   const int64_t blocks = mx::blocks_of(p.cols);
   const int block = chunk / (mx::BLOCK / EACH);
   if (there && block < blocks) *reinterpret_cast<uint32_t *>(p.codes + row * blocks * 16 + chunk * 4) = word;
-  if ((threadIdx.x & 3) == 0) p.scales[mx::scale_at(row, block, p.tiles)] = static_cast<uint8_t>(there && block < blocks ? scale : 0);
+  // four blocks' scales make a word of their tile
+  const uint32_t half = 0xffffu << (threadIdx.x & 16);
+  uint32_t four = there && block < blocks ? scale : 0;
+  four |= __shfl_down_sync(half, four, 4, 16) << 8;
+  four |= __shfl_down_sync(half, four, 8, 16) << 16;
+  if ((threadIdx.x & 15) == 0) *reinterpret_cast<uint32_t *>(p.scales + mx::scale_at(row, block, p.tiles)) = four;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS) dequantize_mxfp4_kernel(const MxParams p) {
   mb_grid_dep_launch();
   mb_grid_dep_wait();
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
-  const int64_t row = item / p.chunks;
-  const int chunk = static_cast<int>(item - row * p.chunks);
+  int64_t row;
+  int chunk;
+  place(p, &row, &chunk);
   const int col = chunk * EACH;
   if (row >= p.rows || col >= p.cols) return;
   const int64_t blocks = mx::blocks_of(p.cols);
@@ -128,6 +151,10 @@ MxParams make(const void *x, void *y, uint8_t *codes, uint8_t *scales, int64_t r
   p.cols = static_cast<int>(cols);
   p.tiles = static_cast<int>(mx::tile_cols(cols));
   p.chunks = p.tiles * (mx::TILE_BLOCKS * mx::BLOCK / EACH);
+  p.block_rows = std::max(1, THREADS / p.chunks);
+  p.row_blocks = (p.chunks + THREADS - 1) / THREADS;
+  fast_div_make(p.chunks, &p.chunk_mul, &p.chunk_shift);
+  fast_div_make(p.row_blocks, &p.row_mul, &p.row_shift);
   const void *values = x != nullptr ? x : y;
   p.vec = kv::aligned(values, 16) && stride * kv::type_bytes(dtype) % 16 == 0;
   return p;
@@ -149,7 +176,7 @@ int mb_quantize_mxfp4(mb_context *ctx, const void *x, uint8_t *codes, uint8_t *s
   if (rows == 0 || cols == 0) return MB_SUCCESS;
   MB_CUDA(ctx, cudaSetDevice(ctx->device));
   const MxParams p = make(x, nullptr, codes, scales, rows, cols, stride, dtype);
-  const int64_t blocks = ceil_div64(mx::tile_rows(rows) * mx::TILE_ROWS * p.chunks, THREADS);
+  const int64_t blocks = ceil_div64(mx::tile_rows(rows) * mx::TILE_ROWS, p.block_rows) * p.row_blocks;
   if (blocks > kv::MOST) return mb_fail(ctx, MB_UNSUPPORTED, "mb_quantize_mxfp4: tensor too large");
   MB_FOR_ELEMENT(dtype, MB_CUDA(ctx, mb_launch_chained(ctx, quantize_mxfp4_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(THREADS), 0, p)));
   ctx->launches++;
@@ -164,7 +191,7 @@ int mb_dequantize_mxfp4(mb_context *ctx, const uint8_t *codes, const uint8_t *sc
   if (rows == 0 || cols == 0) return MB_SUCCESS;
   MB_CUDA(ctx, cudaSetDevice(ctx->device));
   const MxParams p = make(nullptr, x, const_cast<uint8_t *>(codes), const_cast<uint8_t *>(scales), rows, cols, stride, dtype);
-  const int64_t blocks = ceil_div64(rows * p.chunks, THREADS);
+  const int64_t blocks = ceil_div64(rows, p.block_rows) * p.row_blocks;
   if (blocks > kv::MOST) return mb_fail(ctx, MB_UNSUPPORTED, "mb_dequantize_mxfp4: tensor too large");
   MB_FOR_ELEMENT(dtype, MB_CUDA(ctx, mb_launch_chained(ctx, dequantize_mxfp4_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(THREADS), 0, p)));
   ctx->launches++;

@@ -112,6 +112,25 @@ def test_long(ctx, name, batch, heads, kv_heads, dim, longest):
     Case(ctx, name, lengths, heads, kv_heads, dim, 32, seed=batch).run().check()
 
 
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_many_sequences(ctx, name):
+    """More sequences than every block reads the lengths of, short ones and a long one."""
+    rng = np.random.default_rng(8)
+    lengths = [int(n) for n in rng.integers(0, 20, 1100)]
+    lengths[500] = 9000
+    Case(ctx, name, lengths, 4, 2, 64, 16, seed=8).run().check()
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("batch", [127, 128, 129, 300])
+def test_ragged_batches(ctx, name, batch):
+    """Sequences beyond one round of the blocks' sum over lengths, some empty."""
+    rng = np.random.default_rng(batch)
+    lengths = [int(n) for n in rng.integers(0, 300, batch)]
+    lengths[batch // 3], lengths[-1] = 3000, 0
+    Case(ctx, name, lengths, 2, 1, 64, 16, seed=batch, weights=False).run().check()
+
+
 @pytest.mark.parametrize("name", ["f16", "bf16"])
 def test_on_cuda_cores(ctx, name):
     """The kernel of fp32 and odd rows serves 16-bit types too ("tensor_cores" 0)."""
