@@ -16,7 +16,9 @@ MB_HD int64_t tile_cols(int64_t cols) { return (blocks_of(cols) + TILE_BLOCKS - 
 MB_HD int64_t scale_bytes(int64_t rows, int64_t cols) { return tile_rows(rows) * tile_cols(cols) * TILE_BYTES; }
 // Where the scale of row r's block b lies, `tiles` tiles of blocks to a row of tiles.
 MB_HD int64_t scale_at(int64_t r, int64_t b, int64_t tiles) {
-  return (r / TILE_ROWS * tiles + b / TILE_BLOCKS) * TILE_BYTES + r % 32 * 16 + r / 32 % 4 * 4 + b % TILE_BLOCKS;
+  const uint32_t row = static_cast<uint32_t>(r), block = static_cast<uint32_t>(b);   // (both below 2^31)
+  return (static_cast<int64_t>(row / TILE_ROWS) * tiles + block / TILE_BLOCKS) * TILE_BYTES + row % 32 * 16 + row / 32 % 4 * 4 +
+         block % TILE_BLOCKS;
 }
 
 inline kv::Verdict check_tensor(const void *x, const void *codes, const void *scales, int64_t rows, int64_t cols, int64_t stride,

@@ -1,8 +1,8 @@
 // Quantization to 4-bit microscaled floating point (blocks of 32 E2M1 codes that share an E8M0 scale) and back.
 //
-// A thread has eight values, so four neighbouring lanes have a block: its largest magnitude is two shuffles away, and its exponent
-// field is the scale.  Dividing by a power of two is exact, and the conversion rounds to nearest even and saturates, so the result is
-// the definition's bit for bit.
+// A thread has eight values at a time, so four neighbouring lanes have a block: its largest magnitude is two shuffles away, and its
+// exponent field is the scale.  Dividing by a power of two is exact, and the conversion rounds to nearest even and saturates, so the
+// result is the definition's bit for bit.
 #include <algorithm>
 
 #include "elements.cuh"
@@ -11,7 +11,8 @@
 namespace {
 
 constexpr int THREADS = 256;
-constexpr int EACH = 8;   // values of a thread
+constexpr int EACH = 8;    // values of a thread at a time
+constexpr int TIMES = 4;   // groups of them, THREADS apart, so that addresses are worked out once and four loads are in flight
 
 struct MxParams {
   const void *x;
@@ -21,127 +22,188 @@ struct MxParams {
   int cols, tiles;       // tiles of scales in a row of tiles
   int chunks;            // groups of EACH values in a row's tiles
   int vec;               // words of 16 bytes (fp32: two of them) are aligned
-  int block_rows, row_blocks;   // a block has whole rows, or a row whole blocks
+  int block_rows, row_blocks;   // a block has block_rows rows at a time, or (row_blocks > 0) a row so many blocks
   uint32_t chunk_mul, chunk_shift, row_mul, row_shift;
 };
 
+// Eight values as they lie, zeros behind the row's end.
 template <typename T>
-__device__ __forceinline__ void load_eight(const MxParams &p, const T *row, int col, float (&v)[EACH]) {
-  if (p.vec && col + EACH <= p.cols) {
-    constexpr int W = 16 / sizeof(T);
+struct Eight {
+  uint32_t word[EACH * sizeof(T) / 4];
+  __device__ __forceinline__ void load(const MxParams &p, const T *row, int col) {
+    constexpr int WORDS = sizeof(word) / 16;
+    if (p.vec && col + EACH <= p.cols) {
 #pragma unroll
-    for (int w = 0; w < EACH / W; ++w) {
-      elem::Vec<T, W> word;
-      word.load(row + col + w * W);
+      for (int w = 0; w < WORDS; ++w) {
+        const uint4 v = mb_load(reinterpret_cast<const uint4 *>(row + col) + w);
+        word[4 * w] = v.x, word[4 * w + 1] = v.y, word[4 * w + 2] = v.z, word[4 * w + 3] = v.w;
+      }
+    } else {
+      elem::Vec<T, 4 / sizeof(T)> pack;
 #pragma unroll
-      for (int i = 0; i < W; ++i) v[w * W + i] = elem::widen(word.v[i]);
+      for (int w = 0; w < static_cast<int>(sizeof(word) / 4); ++w) {
+        pack.word = 0;
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(4 / sizeof(T)); ++i) {
+          const int at = col + w * (4 / sizeof(T)) + i;
+          if (at < p.cols) pack.v[i] = mb_load(row + at);
+        }
+        word[w] = pack.word;
+      }
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) v[i] = col + i < p.cols ? elem::widen(mb_load(row + col + i)) : 0.f;
   }
-}
+  __device__ __forceinline__ float value(int i) const {
+    elem::Vec<T, 4 / sizeof(T)> pack;
+    pack.word = word[i * sizeof(T) / 4];
+    return elem::widen(pack.v[i % (4 / sizeof(T))]);
+  }
+  // The largest magnitude as fp32 bits (a NaN's are larger than everything).
+  __device__ __forceinline__ uint32_t top() const {
+    if constexpr (sizeof(T) == 4) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) m = max(m, word[i] & 0x7fffffffu);
+      return m;
+    } else {
+      // magnitudes of 16-bit floats order as numbers, two at a time
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < EACH / 2; ++i) m = __vmaxu2(m, word[i] & 0x7fff7fffu);
+      elem::Vec<T, 2> pack;
+      pack.word = max(m & 0xffffu, m >> 16);
+      return __float_as_uint(elem::widen(pack.v[0]));
+    }
+  }
+};
 
-// Two codes of a byte: lo in the low half.
-__device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
-  uint16_t r;
-  asm("{\n\t.reg .b8 c;\n\tcvt.rn.satfinite.e2m1x2.f32 c, %2, %1;\n\tcvt.u16.u8 %0, c;\n\t}" : "=h"(r) : "f"(lo), "f"(hi));
+// Eight codes: the first value in the low half of the first byte.
+__device__ __forceinline__ uint32_t e2m1x8(const float (&v)[EACH]) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
   return r;
 }
 
-// A thread's row and group of eight: with the whole tiles' groups of a row below THREADS a block has several rows, else a row
-// several blocks.  chunk may lie behind the row's last.
-__device__ __forceinline__ void place(const MxParams &p, int64_t *row, int *chunk) {
-  if (p.row_blocks == 1) {
-    const int r = static_cast<int>(fast_div(threadIdx.x, p.chunk_mul, p.chunk_shift));
-    *row = static_cast<int64_t>(blockIdx.x) * p.block_rows + r;
-    *chunk = r < p.block_rows ? static_cast<int>(threadIdx.x) - r * p.chunks : p.chunks;
-  } else {
-    const int r = static_cast<int>(fast_div(blockIdx.x, p.row_mul, p.row_shift));
-    *row = r;
-    *chunk = (static_cast<int>(blockIdx.x) - r * p.row_blocks) * THREADS + threadIdx.x;
-  }
+// The values of two codes, as halves: every one is exact.
+__device__ __forceinline__ float2 values_of(uint32_t byte) {
+  uint32_t h;
+  asm("{\n\t.reg .b8 c;\n\tcvt.u8.u32 c, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, c;\n\t}" : "=r"(h) : "r"(byte));
+  return __half22float2(*reinterpret_cast<const __half2 *>(&h));
 }
 
-// Items are (row, group of eight) of the whole tiles: a lane whose block does not exist writes the tile's zeros.
-template <typename T>
+// Where a thread's groups lie.  WIDE: a row has one or more blocks, and the thread groups chunk, chunk + THREADS, .. of it; else a block
+// has several rows, and the thread the same group of rows block_rows apart.
+template <bool WIDE>
+struct Span {
+  int64_t row;
+  int chunk;
+  __device__ __forceinline__ explicit Span(const MxParams &p) {
+    if (WIDE) {
+      const int r = static_cast<int>(fast_div(blockIdx.x, p.row_mul, p.row_shift));
+      row = r;
+      chunk = (static_cast<int>(blockIdx.x) - r * p.row_blocks) * (THREADS * TIMES) + threadIdx.x;
+    } else {
+      const int r = static_cast<int>(fast_div(threadIdx.x, p.chunk_mul, p.chunk_shift));
+      row = static_cast<int64_t>(blockIdx.x) * p.block_rows * TIMES + r;
+      chunk = r < p.block_rows ? static_cast<int>(threadIdx.x) - r * p.chunks : p.chunks;
+    }
+  }
+  __device__ __forceinline__ int64_t row_of(const MxParams &p, int i) const { return WIDE ? row : row + i * p.block_rows; }
+  __device__ __forceinline__ int chunk_of(int i) const { return WIDE ? chunk + i * THREADS : chunk; }
+};
+
+// Items are (row, group of eight) of the whole tiles: a lane whose block does not exist writes the tile's zeros.  Rows are whole groups
+// of sixteen lanes, whose four scales leave as a word.
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(THREADS) quantize_mxfp4_kernel(const MxParams p) {
   mb_grid_dep_launch();
   mb_grid_dep_wait();
-  int64_t row;
-  int chunk;
-  place(p, &row, &chunk);
-  // (rows are whole groups of sixteen lanes, whose words of four scales leave together)
-  if (chunk >= p.chunks || row >= mx::tile_rows(p.rows) * mx::TILE_ROWS) return;
-  const int col = chunk * EACH;
-  const bool there = row < p.rows;
-  float v[EACH];
+  const Span<WIDE> at(p);
+  const int blocks = static_cast<int>(mx::blocks_of(p.cols));
+  const int64_t tile_rows = mx::tile_rows(p.rows) * mx::TILE_ROWS;
+  Eight<T> x[TIMES];
 #pragma unroll
-  for (int i = 0; i < EACH; ++i) v[i] = 0.f;
-  if (there && col < p.cols) load_eight(p, static_cast<const T *>(p.x) + row * p.stride, col, v);
-  uint32_t top = 0;
+  for (int i = 0; i < TIMES; ++i) {
+    const int64_t row = at.row_of(p, i);
+    const int col = at.chunk_of(i) * EACH;
 #pragma unroll
-  for (int i = 0; i < EACH; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-  const uint32_t lanes = 0xfu << (threadIdx.x & 28);
-  top = max(top, __shfl_xor_sync(lanes, top, 1));
-  top = max(top, __shfl_xor_sync(lanes, top, 2));
-  // floor(log2 max) - 2, at least -127; the biased exponent is that plus 129, 0 for what is below 2^-126
-  const int field = static_cast<int>(top >> 23);
-  int scale = field == 255 ? 255 : max(field - 2, 0);
-  uint32_t word = 0;
-  if (scale != 255) {
+    for (uint32_t &w : x[i].word) w = 0;
+    if (row < p.rows && col < p.cols) x[i].load(p, static_cast<const T *>(p.x) + row * p.stride, col);
+  }
+#pragma unroll
+  for (int i = 0; i < TIMES; ++i) {
+    const int64_t row = at.row_of(p, i);
+    const int chunk = at.chunk_of(i), block = chunk / (mx::BLOCK / EACH);
+    // (all lanes take part in the exchange, also those of the last block whose groups lie behind the row)
+    uint32_t top = x[i].top();
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // floor(log2 max) - 2, at least -127; the biased exponent is that plus 129, 0 for what is below 2^-126
+    const int field = static_cast<int>(top >> 23);
+    const int scale = field == 255 ? 255 : max(field - 2, 0);
     // times 2^(127 - scale): a field of 254 - scale, at scale 0 .. 252 always a normal number
     const float factor = __uint_as_float(static_cast<uint32_t>(254 - scale) << 23);
+    float v[EACH];
 #pragma unroll
-    for (int i = 0; i < EACH; i += 2) word |= e2m1x2(v[i] * factor, v[i + 1] * factor) << (4 * i);
+    for (int j = 0; j < EACH; ++j) v[j] = x[i].value(j) * factor;
+    const uint32_t word = scale == 255 ? 0 : e2m1x8(v);
+    const bool there = row < p.rows && block < blocks;
+    uint32_t four = there ? scale : 0;
+    four |= __shfl_down_sync(0xffffffffu, four, 4, 16) << 8;
+    four |= __shfl_down_sync(0xffffffffu, four, 8, 16) << 16;
+    if (there) reinterpret_cast<uint32_t *>(p.codes + row * blocks * 16)[chunk] = word;
+    if ((threadIdx.x & 15) == 0 && row < tile_rows && chunk < p.chunks)
+      *reinterpret_cast<uint32_t *>(p.scales + mx::scale_at(row, block, p.tiles)) = four;
   }
-  const int64_t blocks = mx::blocks_of(p.cols);
-  const int block = chunk / (mx::BLOCK / EACH);
-  if (there && block < blocks) *reinterpret_cast<uint32_t *>(p.codes + row * blocks * 16 + chunk * 4) = word;
-  // four blocks' scales make a word of their tile
-  const uint32_t half = 0xffffu << (threadIdx.x & 16);
-  uint32_t four = there && block < blocks ? scale : 0;
-  four |= __shfl_down_sync(half, four, 4, 16) << 8;
-  four |= __shfl_down_sync(half, four, 8, 16) << 16;
-  if ((threadIdx.x & 15) == 0) *reinterpret_cast<uint32_t *>(p.scales + mx::scale_at(row, block, p.tiles)) = four;
 }
 
-template <typename T>
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(THREADS) dequantize_mxfp4_kernel(const MxParams p) {
   mb_grid_dep_launch();
   mb_grid_dep_wait();
-  int64_t row;
-  int chunk;
-  place(p, &row, &chunk);
-  const int col = chunk * EACH;
-  if (row >= p.rows || col >= p.cols) return;
-  const int64_t blocks = mx::blocks_of(p.cols);
-  const uint32_t word = mb_load(reinterpret_cast<const uint32_t *>(p.codes + row * blocks * 16) + chunk);
-  const int scale = mb_load(p.scales + mx::scale_at(row, chunk / (mx::BLOCK / EACH), p.tiles));
-  // 2^(scale - 127): scale 0 is the subnormal 2^-127, 255 is NaN
-  const float unit = __uint_as_float(scale == 255 ? 0x7fc00000u : scale == 0 ? 0x00400000u : static_cast<uint32_t>(scale) << 23);
-  T *to = static_cast<T *>(p.y) + row * p.stride + col;
-  T v[EACH];
+  const Span<WIDE> at(p);
+  const int blocks = static_cast<int>(mx::blocks_of(p.cols));
+  uint32_t word[TIMES];
+  int scale[TIMES];
 #pragma unroll
-  for (int i = 0; i < EACH; ++i) {
-    const uint32_t code = word >> (4 * i);
-    // magnitude m (1 + half a bit) 2^(e - 1): bits e and mantissa put under a float's exponent, times 2^126; code 1 is a subnormal there
-    const float value = __uint_as_float((code & 8u) << 28 | (code & 7u) << 22) * 8.507059173023461586e37f;
-    v[i] = elem::narrow<T>(value * unit);
-  }
-  if (p.vec && col + EACH <= p.cols) {
-    constexpr int W = 16 / sizeof(T);
-#pragma unroll
-    for (int w = 0; w < EACH / W; ++w) {
-      elem::Vec<T, W> out;
-#pragma unroll
-      for (int i = 0; i < W; ++i) out.v[i] = v[w * W + i];
-      out.store(to + w * W);
+  for (int i = 0; i < TIMES; ++i) {
+    const int64_t row = at.row_of(p, i);
+    const int chunk = at.chunk_of(i);
+    word[i] = scale[i] = 0;
+    if (row < p.rows && chunk * EACH < p.cols) {
+      word[i] = mb_load(reinterpret_cast<const uint32_t *>(p.codes + row * blocks * 16) + chunk);
+      scale[i] = mb_load(p.scales + mx::scale_at(row, chunk / (mx::BLOCK / EACH), p.tiles));
     }
-  } else {
+  }
 #pragma unroll
-    for (int i = 0; i < EACH; ++i)
-      if (col + i < p.cols) to[i] = v[i];
+  for (int i = 0; i < TIMES; ++i) {
+    const int64_t row = at.row_of(p, i);
+    const int col = at.chunk_of(i) * EACH;
+    if (row >= p.rows || col >= p.cols) continue;
+    // 2^(scale - 127): scale 0 is the subnormal 2^-127, 255 is NaN
+    const float unit = __uint_as_float(scale[i] == 255 ? 0x7fc00000u : scale[i] == 0 ? 0x00400000u : static_cast<uint32_t>(scale[i]) << 23);
+    T *to = static_cast<T *>(p.y) + row * p.stride + col;
+    constexpr int W = 16 / sizeof(T);
+    elem::Vec<T, W> out[EACH / W];
+#pragma unroll
+    for (int j = 0; j < EACH; j += 2) {
+      const float2 v = values_of(word[i] >> (4 * j) & 0xffu);
+      out[j / W].v[j % W] = elem::narrow<T>(v.x * unit);
+      out[j / W].v[j % W + 1] = elem::narrow<T>(v.y * unit);
+    }
+    if (p.vec && col + EACH <= p.cols) {
+#pragma unroll
+      for (int w = 0; w < EACH / W; ++w) out[w].store(to + w * W);
+    } else {
+#pragma unroll
+      for (int j = 0; j < EACH; ++j)
+        if (col + j < p.cols) to[j] = out[j / W].v[j % W];
+    }
   }
 }
 
@@ -151,13 +213,18 @@ MxParams make(const void *x, void *y, uint8_t *codes, uint8_t *scales, int64_t r
   p.cols = static_cast<int>(cols);
   p.tiles = static_cast<int>(mx::tile_cols(cols));
   p.chunks = p.tiles * (mx::TILE_BLOCKS * mx::BLOCK / EACH);
+  // a row of THREADS groups or more has blocks of its own; shorter ones share one
   p.block_rows = std::max(1, THREADS / p.chunks);
-  p.row_blocks = (p.chunks + THREADS - 1) / THREADS;
+  p.row_blocks = p.chunks < THREADS ? 0 : (p.chunks + THREADS * TIMES - 1) / (THREADS * TIMES);
   fast_div_make(p.chunks, &p.chunk_mul, &p.chunk_shift);
   fast_div_make(p.row_blocks, &p.row_mul, &p.row_shift);
   const void *values = x != nullptr ? x : y;
   p.vec = kv::aligned(values, 16) && stride * kv::type_bytes(dtype) % 16 == 0;
   return p;
+}
+
+int64_t blocks_for(const MxParams &p, int64_t rows) {
+  return p.row_blocks == 0 ? ceil_div64(rows, static_cast<int64_t>(p.block_rows) * TIMES) : rows * p.row_blocks;
 }
 
 }  // namespace
@@ -176,9 +243,10 @@ int mb_quantize_mxfp4(mb_context *ctx, const void *x, uint8_t *codes, uint8_t *s
   if (rows == 0 || cols == 0) return MB_SUCCESS;
   MB_CUDA(ctx, cudaSetDevice(ctx->device));
   const MxParams p = make(x, nullptr, codes, scales, rows, cols, stride, dtype);
-  const int64_t blocks = ceil_div64(mx::tile_rows(rows) * mx::TILE_ROWS, p.block_rows) * p.row_blocks;
+  const int64_t blocks = blocks_for(p, mx::tile_rows(rows) * mx::TILE_ROWS);
   if (blocks > kv::MOST) return mb_fail(ctx, MB_UNSUPPORTED, "mb_quantize_mxfp4: tensor too large");
-  MB_FOR_ELEMENT(dtype, MB_CUDA(ctx, mb_launch_chained(ctx, quantize_mxfp4_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(THREADS), 0, p)));
+  MB_FOR_ELEMENT(dtype, MB_CUDA(ctx, mb_launch_chained(ctx, p.row_blocks > 0 ? quantize_mxfp4_kernel<T, true> : quantize_mxfp4_kernel<T, false>,
+                                                       dim3(static_cast<unsigned>(blocks)), dim3(THREADS), 0, p)));
   ctx->launches++;
   return MB_SUCCESS;
 }
@@ -191,9 +259,10 @@ int mb_dequantize_mxfp4(mb_context *ctx, const uint8_t *codes, const uint8_t *sc
   if (rows == 0 || cols == 0) return MB_SUCCESS;
   MB_CUDA(ctx, cudaSetDevice(ctx->device));
   const MxParams p = make(nullptr, x, const_cast<uint8_t *>(codes), const_cast<uint8_t *>(scales), rows, cols, stride, dtype);
-  const int64_t blocks = ceil_div64(rows, p.block_rows) * p.row_blocks;
+  const int64_t blocks = blocks_for(p, rows);
   if (blocks > kv::MOST) return mb_fail(ctx, MB_UNSUPPORTED, "mb_dequantize_mxfp4: tensor too large");
-  MB_FOR_ELEMENT(dtype, MB_CUDA(ctx, mb_launch_chained(ctx, dequantize_mxfp4_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(THREADS), 0, p)));
+  MB_FOR_ELEMENT(dtype, MB_CUDA(ctx, mb_launch_chained(ctx, p.row_blocks > 0 ? dequantize_mxfp4_kernel<T, true> : dequantize_mxfp4_kernel<T, false>,
+                                                       dim3(static_cast<unsigned>(blocks)), dim3(THREADS), 0, p)));
   ctx->launches++;
   return MB_SUCCESS;
 }

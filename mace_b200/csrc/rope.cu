@@ -87,14 +87,34 @@ struct Item {
     if (TWO && turns) b.load(src + other(p));
   }
 
+  static constexpr int PAIRS = TWO ? V : V / 2;         // that a turning item has
+
+  // Where pair q of a token lies in its table: two of an item's side by side, words of neighbouring items next to each other, so that
+  // lanes read 16 bytes each without meeting in a bank.
+  static __device__ __forceinline__ int table_at(int q, int items) {
+    if (PAIRS == 1) return q;
+    const int j = q / PAIRS, i = q % PAIRS;
+    return ((i / 2) * items + j) * 2 + i % 2;
+  }
+
   __device__ __forceinline__ int other(const RopeParams &p) const { return INTERLEAVED ? at + 1 : at + p.half; }
 
   __device__ __forceinline__ void finish(const RopeParams &p, const float2 *table) {
     if (dst == nullptr) return;
     if (pair >= 0) {
-      const float2 *cs = table + token * p.half + pair;
+      float2 cs[PAIRS];
+      if constexpr (PAIRS == 1) {
+        cs[0] = table[token * p.half + pair];
+      } else {
 #pragma unroll
-      for (int i = 0; i < (TWO ? V : V / 2); ++i) {
+        for (int i = 0; i < PAIRS; i += 2) {
+          const float4 w = *reinterpret_cast<const float4 *>(table + token * p.half + ((i / 2) * p.turning + pair / PAIRS) * 2);
+          cs[i] = make_float2(w.x, w.y);
+          cs[i + 1] = make_float2(w.z, w.w);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) {
         T &lo = TWO ? a.v[i] : a.v[(2 * i) % V], &hi = TWO ? b.v[i] : a.v[(2 * i + 1) % V];
         const float x = elem::widen(lo), y = elem::widen(hi), c = cs[i].x, s = cs[i].y;
         lo = elem::narrow<T>(x * c - y * s);
@@ -110,7 +130,7 @@ template <typename T, int V, bool INTERLEAVED>
 __global__ void __launch_bounds__(THREADS) rope_kernel(const RopeParams p) {
   // two words per item: two items a thread; else four.  64 bytes of a thread's are in flight.
   constexpr int U = Item<T, V, INTERLEAVED>::TWO ? 2 : 4;
-  extern __shared__ float2 table[];
+  extern __shared__ __align__(16) float2 table[];
   mb_grid_dep_launch();
   mb_grid_dep_wait();
   const int64_t token0 = static_cast<int64_t>(blockIdx.x) * p.tokens_per_block;
@@ -123,7 +143,7 @@ __global__ void __launch_bounds__(THREADS) rope_kernel(const RopeParams p) {
     const double turns = mb_load(p.positions + token0 + token) * (mb_load(p.freq + (i - token * p.half)) * 0.15915494309189533577);
     float s, c;
     sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &c);
-    table[i] = make_float2(c * p.cos_factor, s * p.sin_factor);
+    table[token * p.half + Item<T, V, INTERLEAVED>::table_at(i - token * p.half, p.turning)] = make_float2(c * p.cos_factor, s * p.sin_factor);
   }
   __syncthreads();
 #pragma unroll
