@@ -149,7 +149,8 @@ def _check(got, a, b, bias, name, cores=False):
 
 
 SHAPES = [(1, 1, 1), (1, 16, 32), (1, 4096, 4096), (3, 130, 100), (16, 333, 777), (17, 128, 64), (128, 128, 128), (129, 127, 300), (200, 1000, 513),
-          (64, 4099, 256), (513, 640, 1024), (40, 8192, 160), (300, 260, 4096), (1000, 1000, 96)]
+          (64, 4099, 256), (513, 640, 1024), (40, 8192, 160), (300, 260, 4096), (1000, 1000, 96),
+          (2500, 2100, 160), (2563, 2305, 700), (4097, 1280, 64)]
 
 
 @pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
@@ -172,7 +173,7 @@ def test_gemm_on_cuda_cores(ctx, M, N, K):
     _check(_gemm(ctx, a, b, bias, "f32", tensor_cores=0), a, b, bias, "f32", cores=True)
 
 
-@pytest.mark.parametrize("M,N,K", [(1, 128, 256), (20, 130, 512), (300, 520, 256)])
+@pytest.mark.parametrize("M,N,K", [(1, 128, 256), (20, 130, 512), (300, 520, 256), (2400, 2200, 512)])
 def test_gemm_every_code_and_scale_has_its_place(ctx, M, N, K):
     """One non-zero block of one row of each operand: every other result is zero, that one is the block's product.  A scale or code
     that is taken from another row, block or half gives another power of two."""
