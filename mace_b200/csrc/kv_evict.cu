@@ -1,14 +1,18 @@
 // Eviction from a paged cache by accumulated attention weight: of every kv head's slots the heaviest are kept, in order.
 //
 // Two kernels.  The first finds, per sequence and kv head, the weight of the last slot that is kept: a radix selection from the top
-// byte down, on the weights' order-preserving integers.  Above that weight everything stays, of those equal to it the lowest slots; a
+// digit down, on the weights' order-preserving integers.  Above that weight everything stays, of those equal to it the lowest slots; a
 // prefix sum over counts then gives every kept slot its place.  The second copies rows of keys and values.
+#include <algorithm>
+
 #include "elements.cuh"
+#include "gemm_u8_cut.cuh"
 #include "kv_cache.h"
+#include "sm100_ptx.cuh"
 
 namespace {
 
-constexpr int SELECT_THREADS = 1024;
+constexpr int SELECT_THREADS = 512;
 constexpr int SELECT_WARPS = SELECT_THREADS / 32;
 constexpr int COPY_THREADS = 256;
 constexpr int COPY_EACH = 4;   // words a thread has in flight, of keys and of values each
@@ -23,7 +27,8 @@ struct EvictParams {
   int64_t weights_stride, src_pages, dst_pages;
   int kv_heads, dim, page_size, src_max_pages, dst_max_pages, longest, budget, sinks, recent;
   uint32_t page_mul, page_shift;
-  int words, chunks;   // of a row; blocks of a head's rows
+  int cluster, cached;   // CTAs that select for a head; whether a run of weights fits into one's shared memory
+  int words, chunks;     // of a row; blocks of a head's rows
   uint32_t word_mul, word_shift;
   int *status;
 };
@@ -35,88 +40,165 @@ __device__ __forceinline__ uint32_t order_of(float w) {
   return (u & 0x80000000u) != 0 ? ~u : u | 0x80000000u;
 }
 
-__global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const EvictParams p) {
-  __shared__ unsigned count[256];
-  __shared__ unsigned above[SELECT_WARPS], equal[SELECT_WARPS];
-  __shared__ unsigned digit_s, left_s;
+__device__ __forceinline__ unsigned load_remote_u32(uint32_t addr, int rank) {
+  unsigned v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(sm100::mapa_shared(addr, rank)) : "memory");
+  return v;
+}
+
+// A cluster of CTAs per sequence and kv head, each with a run of the candidates, whose order-preserving integers it keeps in shared
+// memory (where they fit: `cached`).  Digits of 11, 11 and 10 bits; every CTA counts its own, after a cluster barrier each adds up all
+// CTAs' counts through distributed shared memory and comes to the same digit.  What bounds it: two passes over counts and a cluster
+// barrier for each digit, about 1 us, not the weights (33333 of them, 4 heads: 39 us with one CTA a head and bytes as digits, SELECT_US here).
+constexpr int DIGIT = 2048, GROUPS = DIGIT / 32;
+
+// The sum over the lanes up to this one.
+__device__ __forceinline__ unsigned upto_lane(unsigned v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const unsigned below = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += below;
+  }
+  return v;
+}
+
+__global__ void __launch_bounds__(SELECT_THREADS, 2) evict_select_kernel(const EvictParams p) {
+  extern __shared__ uint32_t keys[];
+  __shared__ __align__(8) unsigned counts[3][DIGIT], groups[3][GROUPS];
+  __shared__ unsigned above[SELECT_WARPS], equal[SELECT_WARPS], mine[2];
+  __shared__ unsigned digit_s, left_s, held_s;
   mb_grid_dep_launch();
   mb_grid_dep_wait();
-  const int unit = blockIdx.x, batch = unit / p.kv_heads;
+  const int rank = p.cluster > 1 ? static_cast<int>(sm100::cluster_ctarank()) : 0;
+  const int unit = blockIdx.x / p.cluster, batch = unit / p.kv_heads;
   const int t = threadIdx.x, warp = t / 32, lane = t % 32;
   bool bad;
   const int length = kv::usable_length(mb_load(p.lengths + batch), p.longest, &bad);
-  if (bad && t == 0) mb_report_bad_index(p.status);
+  if (bad && t == 0 && rank == 0) mb_report_bad_index(p.status);
   const float *w = p.weights + unit * p.weights_stride;
   int32_t *kept = p.kept + static_cast<int64_t>(unit) * p.budget;
-  float *to = p.dst_weights + static_cast<int64_t>(unit) * p.budget;
-  if (length <= p.budget) {
-    for (int j = t; j < p.budget; j += SELECT_THREADS) {
-      kept[j] = j < length ? j : -1;
-      if (j < length) to[j] = mb_load(w + j);
-    }
+  const int all = p.cluster * SELECT_THREADS, me = rank * SELECT_THREADS + t;
+  if (length <= p.budget) {   // (the whole cluster agrees)
+    for (int64_t j = me; j < p.budget; j += all) kept[j] = j < length ? static_cast<int32_t>(j) : -1;
     return;
   }
   // candidates lie between the first and the last slots that stay in any case
   const int first = p.sinks, end = length - p.recent, places = p.budget - p.sinks - p.recent;
+  const int run = (end - first + p.cluster - 1) / p.cluster;
+  const int from = min(static_cast<int64_t>(first) + static_cast<int64_t>(rank) * run, static_cast<int64_t>(end));
+  const int until = end - from < run ? end : from + run;
+  const auto key = [&](int j) { return p.cached ? keys[j - from] : order_of(mb_load(w + j)); };
   uint32_t limit = 0xffffffffu;   // (no place: nothing is above, and none of the equal ones is taken)
   unsigned ties = 0;
+  for (int i = t; i < 3 * DIGIT; i += SELECT_THREADS) (&counts[0][0])[i] = 0;
+  if (p.cached) {
+    for (int base = from + t; base - t < until; base += 8 * SELECT_THREADS) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = until - base > i * SELECT_THREADS ? mb_load(w + base + i * SELECT_THREADS) : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (until - base > i * SELECT_THREADS) keys[base - from + i * SELECT_THREADS] = order_of(v[i]);
+    }
+  }
+  for (int j = me; j < first; j += all) kept[j] = j;
+  for (int j = me; j < p.recent; j += all) kept[p.budget - p.recent + j] = end + j;
+  __syncthreads();
   if (places > 0) {
     uint32_t prefix = 0, mask = 0;
     unsigned left = places;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (t < 256) count[t] = 0;
-      __syncthreads();
-      for (int j = first + t; j < end; j += SELECT_THREADS) {
-        const uint32_t u = order_of(mb_load(w + j));
-        if ((u & mask) == prefix) atomicAdd(count + ((u >> shift) & 255u), 1u);
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+      const uint32_t digits = pass == 2 ? 1023u : 2047u;
+      unsigned *count = counts[pass];
+      for (int base = from; base < until; base += SELECT_THREADS) {
+        const int j = base + t;
+        const uint32_t u = j < until ? key(j) : 0;
+        const bool counts_in = j < until && (u & mask) == prefix;
+        const uint32_t d = (u >> shift) & digits;
+        // (weights that are all alike would queue at one counter)
+        int same;
+        __match_all_sync(0xffffffffu, counts_in ? d : 0xffffffffu, &same);
+        if (!same) {
+          if (counts_in) atomicAdd(count + d, 1u);
+        } else if (counts_in && lane == 0) {
+          atomicAdd(count + d, 32u);
+        }
       }
       __syncthreads();
+      // sums of 32 digits each, so that what the CTAs read of one another is 64 sums and then 32 counts
+      for (int g = warp; g < GROUPS; g += SELECT_WARPS) {
+        const unsigned sum = __reduce_add_sync(0xffffffffu, count[g * 32 + lane]);
+        if (lane == 0) groups[pass][g] = sum;
+      }
+      if (p.cluster > 1) sm100::cluster_sync_all();
+      else __syncthreads();
       if (warp == 0) {
-        // lane l has digits 255 - 8 l .. 248 - 8 l, so that lanes go from the largest down
-        unsigned mine = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) mine += count[255 - 8 * lane - i];
-        unsigned before = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-          const unsigned v = __shfl_up_sync(0xffffffffu, before, o);
-          if (lane >= o) before += v;
+        // lane l has groups 63 - 2 l and 62 - 2 l, then digit 31 - l of the group that is found: from the largest down
+        const int g = GROUPS - 2 - 2 * lane;
+        unsigned low = 0, high = 0;
+        if (p.cluster > 1) {
+          const uint32_t addr = sm100::smem_u32(&groups[pass][g]);
+#pragma unroll 8
+          for (int s = 0; s < p.cluster; ++s) {
+            unsigned x, y;
+            asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(x), "=r"(y) : "r"(sm100::mapa_shared(addr, s)) : "memory");
+            low += x;
+            high += y;
+          }
+        } else {
+          low = groups[pass][g];
+          high = groups[pass][g + 1];
         }
-        before -= mine;
-        if (before < left && left <= before + mine) {
-          int d = 255 - 8 * lane;
-          while (before + count[d] < left) before += count[d--];
+        unsigned before = upto_lane(low + high, lane) - low - high;
+        const unsigned here = __ballot_sync(0xffffffffu, before < left && left <= before + low + high);
+        const int who = __ffs(here) - 1;
+        const bool upper = left <= before + high;
+        const int group = __shfl_sync(0xffffffffu, upper ? g + 1 : g, who);
+        const unsigned base = __shfl_sync(0xffffffffu, upper ? before : before + high, who);
+        const int d = group * 32 + 31 - lane;
+        unsigned n = 0;
+        if (p.cluster > 1) {
+          const uint32_t addr = sm100::smem_u32(count + d);
+#pragma unroll 8
+          for (int s = 0; s < p.cluster; ++s) n += load_remote_u32(addr, s);
+        } else {
+          n = count[d];
+        }
+        before = base + upto_lane(n, lane) - n;
+        if (before < left && left <= before + n) {
           digit_s = d;
           left_s = left - before;
+          held_s = n;
         }
       }
       __syncthreads();
       prefix |= digit_s << shift;
-      mask |= 255u << shift;
+      mask |= digits << shift;
       left = left_s;
+      // (all that begin with these digits stay: nothing left to tell apart)
+      if (held_s == left && prefix != 0) {
+        limit = prefix - 1;
+        break;
+      }
+      if (pass == 2) {
+        limit = prefix;
+        ties = left;
+      }
     }
-    limit = prefix;
-    ties = left;
   }
-  for (int j = t; j < first; j += SELECT_THREADS) {
-    kept[j] = j;
-    to[j] = mb_load(w + j);
-  }
-  for (int j = t; j < p.recent; j += SELECT_THREADS) {
-    kept[p.budget - p.recent + j] = end + j;
-    to[p.budget - p.recent + j] = mb_load(w + end + j);
-  }
-  // every warp has a run of the candidates: what it holds, then what lies before it, then where its own go
-  const int run = (end - first + SELECT_THREADS - 1) / SELECT_THREADS * 32;
-  const int from = min(first + warp * run, end), until = min(from + run, end);
+  // every warp has a part of the run: what it holds, then what lies before it, then where its own go
+  const int part = (until - from + SELECT_THREADS - 1) / SELECT_THREADS * 32;
+  const int mine_from = min(from + warp * part, until), mine_until = until - mine_from < part ? until : mine_from + part;
   unsigned a = 0, e = 0;
-  for (int j = from + lane; j < until; j += 32) {
-    const uint32_t u = order_of(mb_load(w + j));
+  for (int j = mine_from + lane; j < mine_until; j += 32) {
+    const uint32_t u = key(j);
     a += u > limit;
     e += u == limit;
   }
   a = __reduce_add_sync(0xffffffffu, a);
   e = __reduce_add_sync(0xffffffffu, e);
+  __syncthreads();
   if (lane == 0) {
     above[warp] = a;
     equal[warp] = e;
@@ -127,25 +209,33 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const Evic
     a += above[i];
     e += equal[i];
   }
-  for (int base = from; base < until; base += 32) {
+  if (p.cluster > 1) {
+    if (t == SELECT_THREADS - 32) {   // (the last warp's first lane has all but its own)
+      mine[0] = a + above[warp];
+      mine[1] = e + equal[warp];
+    }
+    sm100::cluster_sync_all();
+    for (int s = 0; s < rank; ++s) {
+      a += load_remote_u32(sm100::smem_u32(&mine[0]), s);
+      e += load_remote_u32(sm100::smem_u32(&mine[1]), s);
+    }
+  }
+  for (int base = mine_from; base < mine_until; base += 32) {
     const int j = base + lane;
-    const float value = j < until ? mb_load(w + j) : 0.f;
-    const uint32_t u = order_of(value);
-    const unsigned more = __ballot_sync(0xffffffffu, j < until && u > limit), same = __ballot_sync(0xffffffffu, j < until && u == limit);
+    const uint32_t u = j < mine_until ? key(j) : 0;
+    const unsigned more = __ballot_sync(0xffffffffu, j < mine_until && u > limit), same = __ballot_sync(0xffffffffu, j < mine_until && u == limit);
     const unsigned lower = (1u << lane) - 1u;
-    const unsigned rank = e + __popc(same & lower);
-    const bool stays = (more >> lane & 1u) != 0 || ((same >> lane & 1u) != 0 && rank < ties);
-    if (stays) {
-      const int at = first + a + __popc(more & lower) + min(rank, ties);
-      kept[at] = j;
-      to[at] = value;
+    const unsigned rank_of = e + __popc(same & lower);
+    if ((more >> lane & 1u) != 0 || ((same >> lane & 1u) != 0 && rank_of < ties)) {
+      kept[first + a + __popc(more & lower) + min(rank_of, ties)] = j;
     }
     a += __popc(more);
     e += __popc(same);
   }
+  if (p.cluster > 1) sm100::cluster_sync_all();   // (no CTA may leave while another reads its counts)
 }
 
-// Rows of keys and values to their new slots, a word per item, and the new lengths (here, because the other kernel reads the old ones
+// Rows of keys and values to their new slots, a word per item, their weights, and the new lengths (here, because the other kernel reads the old ones
 // and the two may be the same memory).
 template <typename Word>
 __global__ void __launch_bounds__(COPY_THREADS) evict_copy_kernel(const EvictParams p) {
@@ -161,37 +251,52 @@ __global__ void __launch_bounds__(COPY_THREADS) evict_copy_kernel(const EvictPar
   const int32_t *src_table = p.src_table + static_cast<int64_t>(batch) * p.src_max_pages;
   const int32_t *dst_table = p.dst_table + static_cast<int64_t>(batch) * p.dst_max_pages;
   const int rows = COPY_THREADS * COPY_EACH / p.words;   // whole rows of a block; at least one
+  // three loads that wait for one another, each for all items at once: slots, pages, rows
+  int slot[COPY_EACH], src_page[COPY_EACH], dst_page[COPY_EACH];
+#pragma unroll
+  for (int i = 0; i < COPY_EACH; ++i) {
+    const int row = static_cast<int>(fast_div(i * COPY_THREADS + threadIdx.x, p.word_mul, p.word_shift));
+    const int64_t j = static_cast<int64_t>(chunk) * rows + row;
+    slot[i] = row < rows && j < p.budget ? mb_load(kept + j) : -1;
+  }
+#pragma unroll
+  for (int i = 0; i < COPY_EACH; ++i) {
+    const int row = static_cast<int>(fast_div(i * COPY_THREADS + threadIdx.x, p.word_mul, p.word_shift));
+    const int j = chunk * rows + row;
+    src_page[i] = slot[i] >= 0 ? mb_load(src_table + fast_div(slot[i], p.page_mul, p.page_shift)) : -1;
+    dst_page[i] = slot[i] >= 0 ? mb_load(dst_table + fast_div(j, p.page_mul, p.page_shift)) : -1;
+  }
   Word k[COPY_EACH], v[COPY_EACH];
+  float weight[COPY_EACH];
   int64_t to[COPY_EACH];
 #pragma unroll
   for (int i = 0; i < COPY_EACH; ++i) {
     const int item = i * COPY_THREADS + threadIdx.x;
-    const int row = static_cast<int>(fast_div(item, p.word_mul, p.word_shift)), word = item - row * p.words;
-    const int64_t j = static_cast<int64_t>(chunk) * rows + row;
-    to[i] = -1;
-    if (row >= rows || j >= p.budget) continue;
-    const int slot = mb_load(kept + j);
-    if (slot < 0) continue;
-    const int from_page = static_cast<int>(fast_div(slot, p.page_mul, p.page_shift));
-    const int to_page = static_cast<int>(fast_div(static_cast<uint32_t>(j), p.page_mul, p.page_shift));
-    const int64_t from = kv::row_offset(mb_load(src_table + from_page), p.src_pages, p.kv_heads, head, p.page_size,
-                                        slot - from_page * p.page_size, p.words);
-    const int64_t at = kv::row_offset(mb_load(dst_table + to_page), p.dst_pages, p.kv_heads, head, p.page_size,
-                                      static_cast<int>(j) - to_page * p.page_size, p.words);
-    if (from < 0 || at < 0) {
-      mb_report_bad_index(p.status);
-      continue;
+    const int row = static_cast<int>(fast_div(item, p.word_mul, p.word_shift)), word = item - row * p.words, j = chunk * rows + row;
+    const int at_slot = max(slot[i], 0);
+    const int64_t from = kv::row_offset(src_page[i], p.src_pages, p.kv_heads, head, p.page_size,
+                                        at_slot - static_cast<int>(fast_div(at_slot, p.page_mul, p.page_shift)) * p.page_size, p.words);
+    const int64_t at = kv::row_offset(dst_page[i], p.dst_pages, p.kv_heads, head, p.page_size,
+                                      j - static_cast<int>(fast_div(j, p.page_mul, p.page_shift)) * p.page_size, p.words);
+    const bool there = from >= 0 && at >= 0;
+    if (!there && slot[i] >= 0) mb_report_bad_index(p.status);
+    to[i] = there ? at + word : -1;
+    if (there) {
+      k[i] = mb_load(static_cast<const Word *>(p.k_src) + from + word);
+      v[i] = mb_load(static_cast<const Word *>(p.v_src) + from + word);
     }
-    to[i] = at + word;
-    k[i] = mb_load(static_cast<const Word *>(p.k_src) + from + word);
-    v[i] = mb_load(static_cast<const Word *>(p.v_src) + from + word);
+    if (slot[i] >= 0 && word == 0) weight[i] = mb_load(p.weights + unit * p.weights_stride + slot[i]);
   }
 #pragma unroll
-  for (int i = 0; i < COPY_EACH; ++i)
+  for (int i = 0; i < COPY_EACH; ++i) {
+    const int item = i * COPY_THREADS + threadIdx.x;
+    const int row = static_cast<int>(fast_div(item, p.word_mul, p.word_shift));
+    if (slot[i] >= 0 && item == row * p.words) p.dst_weights[static_cast<int64_t>(unit) * p.budget + chunk * rows + row] = weight[i];
     if (to[i] >= 0) {
       static_cast<Word *>(p.k_dst)[to[i]] = k[i];
       static_cast<Word *>(p.v_dst)[to[i]] = v[i];
     }
+  }
 }
 
 template <typename Word>
@@ -239,7 +344,21 @@ extern "C" int mb_kv_evict(mb_context *ctx, const void *k_src, const void *v_src
                          reinterpret_cast<uintptr_t>(v_dst) | static_cast<uintptr_t>(row_bytes);
   if (row_bytes / (bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 2) > COPY_THREADS * COPY_EACH)
     return mb_fail(ctx, MB_UNSUPPORTED, "mb_kv_evict: head_dim too large");
-  MB_CUDA(ctx, mb_launch_chained(ctx, evict_select_kernel, dim3(static_cast<unsigned>(units)), dim3(SELECT_THREADS), 0, p));
+  // two CTAs an SM, and 2048 weights or more to each
+  constexpr int MOST_KEYS = 20 << 10;   // (two CTAs' runs fit)
+  p.cluster = 1;
+  while (p.cluster < 16 && units * p.cluster * 2 <= 2 * ctx->num_sms && p.longest > 2048 * p.cluster) p.cluster *= 2;
+  while (p.cluster < 16 && p.longest > MOST_KEYS * p.cluster) p.cluster *= 2;
+  const int64_t keys = ceil_div64(p.longest, p.cluster);
+  p.cached = keys <= MOST_KEYS;
+  if (units * p.cluster > kv::MOST) return mb_fail(ctx, MB_UNSUPPORTED, "mb_kv_evict: too many kv heads");
+  if (!ctx->evict_attr_set) {
+    MB_CUDA(ctx, cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_KEYS * 4));
+    MB_CUDA(ctx, cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));   // clusters of 16
+    ctx->evict_attr_set = true;
+  }
+  MB_CUDA(ctx, mb_launch_clusters(ctx, evict_select_kernel, static_cast<unsigned>(units * p.cluster), SELECT_THREADS,
+                                  p.cached ? static_cast<size_t>(keys) * 4 : 0, p.cluster, p));
   ctx->launches++;
   if (bits % 16 == 0) return launch_copy<uint4>(ctx, p, units, row_bytes);
   if (bits % 4 == 0) return launch_copy<uint32_t>(ctx, p, units, row_bytes);
