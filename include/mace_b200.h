@@ -552,7 +552,8 @@ int mb_rope_kv_append(mb_context *ctx, const void *q, void *q_out,
  * receives weights_in[j] (0 where weights_in is NULL; weights_in ==
  * weights_out is allowed) plus the sum of p_j over the query heads that kv
  * head h serves; slots outside the window receive weights_in alone, entries
- * from lengths[b] on stay as they are.  head_dim up to 256. */
+ * from lengths[b] on stay as they are.  head_dim up to 256.  An infinite
+ * value (not key) in a slot that counts gives NaN or an infinity. */
 int mb_paged_attention(mb_context *ctx, const void *q, const void *k_cache,
                        const void *v_cache, const int32_t *page_table,
                        const int32_t *lengths, void *out, float *lse,

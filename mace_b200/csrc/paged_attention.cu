@@ -60,8 +60,13 @@ struct Place {
     *from = *first / chunk * chunk;
     return length - *from;
   }
-  static __device__ __forceinline__ int runs_of(const AttentionParams &p, int slots, int run) {
-    return max(1, static_cast<int>((static_cast<unsigned>(slots) + run - 1) / run));
+  // The runs of a sequence, at most *run slots each, made as long as one another.
+  static __device__ __forceinline__ int runs_of(int slots, int *run) {
+    const unsigned n = static_cast<unsigned>(slots), most = static_cast<unsigned>(*run);
+    const unsigned runs = max(1u, (n + most - 1) / most);
+    const unsigned each = max(((n + runs - 1) / runs + 63) / 64 * 64, 64u);
+    *run = static_cast<int>(each);
+    return static_cast<int>(max(1u, (n + each - 1) / each));
   }
 
   // false: there is no such run.
@@ -99,9 +104,10 @@ struct Place {
       batch = x / p.fixed_runs / p.kv_heads;
       const int slots = slots_of(p, batch, chunk, &first, &from, &bad);
       if (bad && t == 0) mb_report_bad_index(p.status);
-      active = runs_of(p, slots, p.fixed_run);
+      int run = p.fixed_run;
+      active = runs_of(slots, &run);
       if (split >= active) return false;
-      place(p, rows, block, from, slots, p.fixed_run);
+      place(p, rows, block, from, slots, run);
       return true;
     }
     long long total = 0;
@@ -116,14 +122,15 @@ struct Place {
     total = 0;
     for (int w = 0; w < WARPS; ++w) total += sums[w];
     const long long share = (total * per_run + p.resident - 1) / p.resident;
-    const int run = static_cast<int>(min(max(static_cast<long long>(LEAST_RUN), (share + 63) / 64 * 64), 0x7fffffc0ll));
+    const int most = static_cast<int>(min(max(static_cast<long long>(LEAST_RUN), (share + 63) / 64 * 64), 0x7fffffc0ll));
     int before = 0;   // runs of the sequences in front of this round's
     for (int base = 0; base < p.batch; base += THREADS) {
       const int b = base + t;
       int slots = 0, mine = 0;
       if (b < p.batch) {
         slots = slots_of(p, b, chunk, &first, &from, &bad);
-        mine = runs_of(p, slots, run) * per_run;
+        int run = most;
+        mine = runs_of(slots, &run) * per_run;
       }
       int upto = mine;
 #pragma unroll
@@ -151,7 +158,8 @@ struct Place {
     if (static_cast<int>(blockIdx.x) >= before) return false;
     batch = found[0];
     const int slots = slots_of(p, batch, chunk, &first, &from, &bad);
-    active = runs_of(p, slots, run);
+    int run = most;
+    active = runs_of(slots, &run);
     // (blocks of heads that share a run follow one another, so that the run comes from memory once)
     int x = blockIdx.x - found[1];
     const int block = x % p.blocks;
@@ -543,6 +551,19 @@ template <> struct Mma<__nv_bfloat16> {
   }
 };
 
+template <> struct Mma<float> {
+  // tf32, 8 of the depth
+  static __device__ __forceinline__ void run(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  // x as a tf32 number and what that leaves, whose own tf32 part ends at 2^-21 of x (of an infinity: NaN)
+  static __device__ __forceinline__ void split(uint32_t x, uint32_t &hi, uint32_t &lo) {
+    hi = x & 0xffffe000u;
+    lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
+  }
+};
+
 template <bool TRANS>
 __device__ __forceinline__ void load_matrices(uint32_t addr, uint32_t (&r)[4]) {
   if (TRANS)
@@ -567,26 +588,37 @@ __device__ __forceinline__ void copy_word(uint32_t dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
-template <int DIM>
+template <typename T, int DIM>
 struct Ring {
-  static constexpr int CHUNK = 16;                            // slots
-  static constexpr int ROW = DIM * 2, WORDS = DIM / 8;        // bytes of a row, its 16-byte words
-  static constexpr int PART = CHUNK * ROW, STAGE = 2 * PART;  // keys, then values
-  static constexpr int STAGES = DIM == 128 ? 2 : 3;
+  static constexpr int CHUNK = 16;                                // slots
+  static constexpr int ROW = DIM * sizeof(T), WORDS = ROW / 16;   // bytes of a row, its 16-byte words
+  static constexpr int EACH = 16 / sizeof(T);                     // values of a word
+  static constexpr int PART = CHUNK * ROW, STAGE = 2 * PART;      // keys, then values
+  static constexpr int STAGES = ROW == 256 ? 2 : 3;               // (two of 256-byte rows: three blocks an SM)
   static constexpr int BYTES = WARPS * STAGES * STAGE;
   static constexpr int PITCH = DIM + 4;                       // floats between rows of the accumulators at the end
   static_assert(2 * 16 * MAX_SPLITS * 4 <= BYTES, "what joins the runs reuses it too");
   static_assert(WARPS * 16 * PITCH * 4 <= BYTES, "accumulators reuse the ring");
 };
 
+// Where the words of a row of values lie: 16-bit rows are read by ldmatrix, eight at a time; fp32 ones as single values, four rows of two
+// words at a time.
+template <bool F32>
+__device__ __forceinline__ int value_swizzle(int r) {
+  return F32 ? (r * 2 & 7) | (r >> 2 & 1) : r & 7;
+}
+
 // HEADS: tiles of 8 query heads.  WHOLE: a chunk of slots lies in one page, and rows have DIM values.
 template <typename T, int DIM, int HEADS, bool WHOLE>
 __global__ void __launch_bounds__(THREADS) paged_attention_mma_kernel(const AttentionParams p) {
-  using G = Ring<DIM>;
-  constexpr int R = 8 * HEADS, CHUNK = G::CHUNK, DIM_STEPS = DIM / 16, STAGES = G::STAGES;
+  using G = Ring<T, DIM>;
+  constexpr bool F32 = sizeof(T) == 4;
+  constexpr int R = 8 * HEADS, CHUNK = G::CHUNK, STAGES = G::STAGES;
+  constexpr int STEPS = G::WORDS / 2, DIM_STEPS = DIM / 16;   // of a product with the keys (two words of a row), with the values
   extern __shared__ __align__(1024) uint8_t ring[];
   __shared__ unsigned valid[WARPS][STAGES];
   __shared__ float top_s[WARPS * R], sum_s[WARPS * R], coef[WARPS * R], total[2 * R];
+  __shared__ __align__(16) float weight_s[F32 ? WARPS : 1][CHUNK][8];   // a chunk's probabilities, to be read as the other operand
   mb_grid_dep_launch();
   mb_grid_dep_wait();
   Place at;
@@ -614,13 +646,13 @@ __global__ void __launch_bounds__(THREADS) paged_attention_mma_kernel(const Atte
     if (chunk < chunks) {
       const uint32_t to = mine + stage * G::STAGE + line * G::ROW;
       if (WHOLE && where >= 0) {
-        const T *ks = k + where + line * DIM + word * 8, *vs = v + where + line * DIM + word * 8;
+        const T *ks = k + where + line * DIM + word * G::EACH, *vs = v + where + line * DIM + word * G::EACH;
         if (lane == 0) valid[warp][stage] = 0xffffu;
 #pragma unroll
         for (int i = 0; i < CHUNK / LINES; ++i) {
-          const uint32_t dst = to + i * LINES * G::ROW + ((word ^ ((i * LINES + line) & 7)) << 4);
-          copy_word(dst, ks + i * LINES * DIM);
-          copy_word(dst + G::PART, vs + i * LINES * DIM);
+          const int r = i * LINES + line;
+          copy_word(to + i * LINES * G::ROW + ((word ^ (r & 7)) << 4), ks + i * LINES * DIM);
+          copy_word(to + i * LINES * G::ROW + G::PART + ((word ^ value_swizzle<F32>(r)) << 4), vs + i * LINES * DIM);
         }
       } else {
         if (WHOLE) where = slot_of(chunk);
@@ -629,11 +661,11 @@ __global__ void __launch_bounds__(THREADS) paged_attention_mma_kernel(const Atte
 #pragma unroll
         for (int i = 0; i < CHUNK / LINES; ++i) {
           const int64_t from = __shfl_sync(0xffffffffu, where, i * LINES + line);
-          const bool there = from >= 0 && word * 8 < p.dim;
-          const int64_t src = there ? from + word * 8 : 0;
-          const uint32_t dst = to + i * LINES * G::ROW + ((word ^ ((i * LINES + line) & 7)) << 4);
-          copy_word(dst, k + src, there ? 16 : 0);
-          copy_word(dst + G::PART, v + src, there ? 16 : 0);
+          const bool there = from >= 0 && word * G::EACH < p.dim;
+          const int64_t src = there ? from + word * G::EACH : 0;
+          const int r = i * LINES + line;
+          copy_word(to + i * LINES * G::ROW + ((word ^ (r & 7)) << 4), k + src, there ? 16 : 0);
+          copy_word(to + i * LINES * G::ROW + G::PART + ((word ^ value_swizzle<F32>(r)) << 4), v + src, there ? 16 : 0);
         }
       }
     }
@@ -643,23 +675,24 @@ __global__ void __launch_bounds__(THREADS) paged_attention_mma_kernel(const Atte
   for (int s = 0; s < STAGES - 1; ++s) fetch(warp + s * WARPS, s, offset_of(warp + s * WARPS));
   int64_t ahead = offset_of(warp + (STAGES - 1) * WARPS);
 
-  // the queries: head `row` of each tile
-  uint32_t q[HEADS][DIM_STEPS][2];
+  // the queries: head `row` of each tile; fp32 ones as they are, split where they are used
+  uint32_t q[HEADS][STEPS][2];
 #pragma unroll
   for (int t = 0; t < HEADS; ++t)
 #pragma unroll
-    for (int s = 0; s < DIM_STEPS; ++s)
+    for (int s = 0; s < STEPS; ++s)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int h = t * 8 + row, d = s * 16 + i * 8 + pair * 2;
-        elem::Vec<T, 2> two;
-        two.word = 0;
+        constexpr int N = 4 / sizeof(T);
+        const int h = t * 8 + row, d = s * 2 * G::EACH + i * G::EACH + pair * N;
+        elem::Vec<T, N> part;
+        part.word = 0;
         if (h < at.heads && d < p.dim) {
           const T *src = static_cast<const T *>(p.q) + at.batch * p.q_stride + static_cast<int64_t>(at.head0 + h) * p.dim + d;
-          two.v[0] = mb_load(src);
-          two.v[1] = mb_load(src + 1);
+#pragma unroll
+          for (int j = 0; j < N; ++j) part.v[j] = mb_load(src + j);
         }
-        q[t][s][i] = two.word;
+        q[t][s][i] = part.word;
       }
   // heads 2 pair and 2 pair + 1 of each tile: values row and row + 8 of every 16, maximum, and this lane's part of the sum
   float acc[HEADS][DIM_STEPS][4], top[HEADS][2], sum[HEADS][2];
@@ -678,7 +711,9 @@ __global__ void __launch_bounds__(THREADS) paged_attention_mma_kernel(const Atte
 #pragma unroll
   for (int d = 0; d < 4; ++d) {
     key_word[d] = key_row + (((2 * d + lane / 16) ^ (lane & 7)) << 4);
-    value_word[d] = value_row + (((2 * d + lane / 8 % 2) ^ (lane & 7)) << 4);
+    // fp32: value `row` (+ 8: d & 1) of every 16 and slot `pair` (+ 4: d & 2) of every 8; every other 16 four words on
+    value_word[d] = F32 ? (pair + d / 2 * 4) * G::ROW + (((row / 4 + d % 2 * 2) ^ value_swizzle<F32>(pair + d / 2 * 4)) << 4) + row % 4 * 4
+                        : value_row + (((2 * d + lane / 8 % 2) ^ (lane & 7)) << 4);
   }
 
   int stage = 0;
@@ -696,11 +731,40 @@ __global__ void __launch_bounds__(THREADS) paged_attention_mma_kernel(const Atte
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[t][j] = 0.f;
 #pragma unroll
-    for (int d = 0; d < DIM_STEPS; ++d) {
+    for (int d = 0; d < STEPS; ++d) {
       uint32_t a[4];
       load_matrices<false>(keys + key_word[d % 4] + d / 4 * 128, a);
+      if constexpr (F32) {
+        uint32_t hi[4], lo[4], qh[2], ql[2];
 #pragma unroll
-      for (int t = 0; t < HEADS; ++t) Mma<T>::run(s[t], a, q[t][d][0], q[t][d][1]);
+        for (int i = 0; i < 4; ++i) Mma<T>::split(a[i], hi[i], lo[i]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) Mma<T>::split(q[0][d][i], qh[i], ql[i]);
+        Mma<T>::run(s[0], hi, ql[0], ql[1]);
+        Mma<T>::run(s[0], lo, qh[0], qh[1]);
+        Mma<T>::run(s[0], hi, qh[0], qh[1]);
+      } else {
+#pragma unroll
+        for (int t = 0; t < HEADS; ++t) Mma<T>::run(s[t], a, q[t][d][0], q[t][d][1]);
+      }
+    }
+    if constexpr (F32) {
+      // NaN: an infinite key or query, which a pair of tf32 numbers does not hold, or one that is NaN.  Once more, by the definition.
+      if (__any_sync(0xffffffffu, s[0][0] != s[0][0] || s[0][1] != s[0][1] || s[0][2] != s[0][2] || s[0][3] != s[0][3])) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int h = pair * 2 + j % 2, r = row + j / 2 * 8;
+          const T *src = static_cast<const T *>(p.q) + at.batch * p.q_stride + static_cast<int64_t>(at.head0 + h) * p.dim;
+          float dot = 0.f;
+          for (int d = 0; d < p.dim && h < at.heads; ++d) {
+            float x;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(keys + r * G::ROW + ((d / 4 ^ (r & 7)) << 4) + d % 4 * 4) : "memory");
+            dot += x * elem::widen(mb_load(src + d));
+          }
+          s[0][j] = dot;
+        }
+        __syncwarp();
+      }
     }
 #pragma unroll
     for (int t = 0; t < HEADS; ++t)
@@ -752,28 +816,63 @@ __global__ void __launch_bounds__(THREADS) paged_attention_mma_kernel(const Atte
           }
         }
     }
-    uint32_t hi[HEADS][2], lo[HEADS][2];
-#pragma unroll
-    for (int t = 0; t < HEADS; ++t) {
-      const float m0 = top[t][0] == -INFINITY ? 0.f : top[t][0], m1 = top[t][1] == -INFINITY ? 0.f : top[t][1];
+    if constexpr (F32) {
+      // probabilities to the other operand's place, by way of shared memory
+      const float m0 = top[0][0] == -INFINITY ? 0.f : top[0][0], m1 = top[0][1] == -INFINITY ? 0.f : top[0][1];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float x = exp2f(s[t][2 * i] - m0), y = exp2f(s[t][2 * i + 1] - m1);
-        sum[t][0] += x;
-        sum[t][1] += y;
-        Mma<T>::split(x, y, hi[t][i], lo[t][i]);
-        hi[t][i] = transposed(hi[t][i]);
-        lo[t][i] = transposed(lo[t][i]);
+        const float x = exp2f(s[0][2 * i] - m0), y = exp2f(s[0][2 * i + 1] - m1);
+        sum[0][0] += x;
+        sum[0][1] += y;
+        *reinterpret_cast<float2 *>(&weight_s[warp][row + 8 * i][2 * pair]) = make_float2(x, y);
       }
-    }
+      __syncwarp();
 #pragma unroll
-    for (int d = 0; d < DIM_STEPS; ++d) {
-      uint32_t a[4];
-      load_matrices<true>(values + value_word[d % 4] + d / 4 * 128, a);
+      for (int half = 0; half < 2; ++half) {   // eight slots
+        uint32_t ph[2], pl[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) Mma<T>::split(__float_as_uint(weight_s[warp][half * 8 + i * 4 + pair][row]), ph[i], pl[i]);
+#pragma unroll
+        for (int d = 0; d < DIM_STEPS; ++d) {
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            // (the swizzle's low three bits: every other 16 values are four words on)
+            const uint32_t addr = values + half * 8 * G::ROW + ((value_word[i] ^ (d % 2 << 6)) + d / 2 * 128);
+            uint32_t x;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(addr) : "memory");
+            Mma<T>::split(x, hi[i], lo[i]);
+          }
+          Mma<T>::run(acc[0][d], hi, pl[0], pl[1]);
+          Mma<T>::run(acc[0][d], lo, ph[0], ph[1]);
+          Mma<T>::run(acc[0][d], hi, ph[0], ph[1]);
+        }
+      }
+      __syncwarp();
+    } else {
+      uint32_t hi[HEADS][2], lo[HEADS][2];
 #pragma unroll
       for (int t = 0; t < HEADS; ++t) {
-        Mma<T>::run(acc[t][d], a, hi[t][0], hi[t][1]);
-        Mma<T>::run(acc[t][d], a, lo[t][0], lo[t][1]);
+        const float m0 = top[t][0] == -INFINITY ? 0.f : top[t][0], m1 = top[t][1] == -INFINITY ? 0.f : top[t][1];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float x = exp2f(s[t][2 * i] - m0), y = exp2f(s[t][2 * i + 1] - m1);
+          sum[t][0] += x;
+          sum[t][1] += y;
+          Mma<T>::split(x, y, hi[t][i], lo[t][i]);
+          hi[t][i] = transposed(hi[t][i]);
+          lo[t][i] = transposed(lo[t][i]);
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < DIM_STEPS; ++d) {
+        uint32_t a[4];
+        load_matrices<true>(values + value_word[d % 4] + d / 4 * 128, a);
+#pragma unroll
+        for (int t = 0; t < HEADS; ++t) {
+          Mma<T>::run(acc[t][d], a, hi[t][0], hi[t][1]);
+          Mma<T>::run(acc[t][d], a, lo[t][0], lo[t][1]);
+        }
       }
     }
     stage = stage + 1 == STAGES ? 0 : stage + 1;
@@ -810,26 +909,29 @@ int launch_mma(mb_context *ctx, const AttentionParams &p, unsigned grid, int ind
   const auto kern = paged_attention_mma_kernel<T, DIM, HEADS, WHOLE>;
   index += (HEADS - 1) * 2 + WHOLE;
   if (!(ctx->attention_attr_mask & (1u << index))) {
-    MB_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<DIM>::BYTES));
+    MB_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<T, DIM>::BYTES));
     MB_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));   // clusters of 16
     ctx->attention_attr_mask |= 1u << index;
   }
-  MB_CUDA(ctx, mb_launch_clusters(ctx, kern, grid, THREADS, Ring<DIM>::BYTES, p.cluster, p));
+  MB_CUDA(ctx, mb_launch_clusters(ctx, kern, grid, THREADS, Ring<T, DIM>::BYTES, p.cluster, p));
   return MB_SUCCESS;
 }
 
 template <typename T, int DIM>
 int launch_mma(mb_context *ctx, const AttentionParams &p, unsigned grid, int rows, int index) {
-  const bool whole = p.dim == DIM && p.page_size % Ring<DIM>::CHUNK == 0;
-  if (rows > 8) return whole ? launch_mma<T, DIM, 2, true>(ctx, p, grid, index) : launch_mma<T, DIM, 2, false>(ctx, p, grid, index);
+  const bool whole = p.dim == DIM && p.page_size % Ring<T, DIM>::CHUNK == 0;
+  if constexpr (sizeof(T) == 2) {
+    if (rows > 8) return whole ? launch_mma<T, DIM, 2, true>(ctx, p, grid, index) : launch_mma<T, DIM, 2, false>(ctx, p, grid, index);
+  }
   return whole ? launch_mma<T, DIM, 1, true>(ctx, p, grid, index) : launch_mma<T, DIM, 1, false>(ctx, p, grid, index);
 }
 
 template <typename T>
 int launch_mma(mb_context *ctx, const AttentionParams &p, unsigned grid, int rows, int index) {
   if (p.dim <= 64) return launch_mma<T, 64>(ctx, p, grid, rows, index);
-  if (p.dim <= 128) return launch_mma<T, 128>(ctx, p, grid, rows, index + 4);
-  return launch_mma<T, 256>(ctx, p, grid, rows, index + 8);
+  if (sizeof(T) == 4 || p.dim <= 128) return launch_mma<T, 128>(ctx, p, grid, rows, index + 4);
+  if constexpr (sizeof(T) == 2) return launch_mma<T, 256>(ctx, p, grid, rows, index + 8);
+  return MB_SUCCESS;
 }
 
 // What each slot has received of the query heads' probabilities, on top of what it had.  Four slots a thread: a word of every head's
@@ -908,8 +1010,10 @@ extern "C" int mb_paged_attention(mb_context *ctx, const void *q, const void *k_
   p.scale2 = scale * LOG2E;
   p.status = ctx->dev_status;
 
-  const bool by_mma = dtype != MB_F32 && ctx->use_tensor_cores && head_dim % 8 == 0 && kv::aligned(k_cache, 16) && kv::aligned(v_cache, 16);
-  const int rows = by_mma ? (p.group > 8 ? 16 : 8) : p.group >= 5 ? 8 : p.group >= 3 ? 4 : p.group;
+  const bool f32 = dtype == MB_F32;
+  const bool by_mma = ctx->use_tensor_cores && head_dim % (f32 ? 4 : 8) == 0 && (!f32 || head_dim <= 128) && kv::aligned(k_cache, 16) &&
+                      kv::aligned(v_cache, 16);
+  const int rows = by_mma ? (p.group > 8 && !f32 ? 16 : 8) : p.group >= 5 ? 8 : p.group >= 3 ? 4 : p.group;
   p.blocks = (p.group + rows - 1) / rows;
   p.batch = static_cast<int>(batch);
   p.pitch = static_cast<int>(align_up(p.dim, 4));
@@ -923,7 +1027,7 @@ extern "C" int mb_paged_attention(mb_context *ctx, const void *q, const void *k_
   p.cluster = 1;
   if (units * p.longest * 2 * head_dim * kv::type_bytes(dtype) <= SMALL)
     while (p.cluster < most && units * p.cluster * 2 <= 2 * ctx->num_sms && p.longest > LEAST_RUN * p.cluster) p.cluster *= 2;
-  const int per_sm = !by_mma ? (rows * p.dim >= 1024 ? 3 : 5) : p.dim > 128 ? 1 : 3;
+  const int per_sm = !by_mma ? (rows * p.dim >= 1024 ? 3 : 5) : p.dim * kv::type_bytes(dtype) > 256 ? 1 : p.dim * kv::type_bytes(dtype) > 128 ? 3 : 4;
   const int64_t slots = per_sm * ctx->num_sms;
   // one round of blocks where the heads leave it room, else several, so that the last one is a small part
   p.resident = static_cast<int>(std::min<int64_t>(units * 2 <= slots ? slots - units : 4 * slots, MAX_SPLITS * kv_heads * p.blocks));
@@ -961,7 +1065,8 @@ extern "C" int mb_paged_attention(mb_context *ctx, const void *q, const void *k_
   const unsigned grid = static_cast<unsigned>(runs);
   cudaError_t e = cudaSuccess;
   if (by_mma) {
-    if (dtype == MB_F16) MB_RETURN_IF_ERROR(launch_mma<__half>(ctx, p, grid, rows, 0));
+    if (f32) MB_RETURN_IF_ERROR(launch_mma<float>(ctx, p, grid, rows, 24));
+    else if (dtype == MB_F16) MB_RETURN_IF_ERROR(launch_mma<__half>(ctx, p, grid, rows, 0));
     else MB_RETURN_IF_ERROR(launch_mma<__nv_bfloat16>(ctx, p, grid, rows, 12));
   } else MB_FOR_ELEMENT(dtype, {
     const uintptr_t word = 4 * sizeof(T);

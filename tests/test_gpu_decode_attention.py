@@ -54,6 +54,7 @@ class Case:
         largest logit's terms (16-bit products on the tensor cores are exact, their sums cut off at 2^-23: the same).  A
         probability is off by twice that (its own logit and the sum), and by the sums over slots: a warp adds a quarter of a run at most,
         then warps and runs, each 2^-23 at most.  16-bit probabilities are kept as pairs of values: 2^-16 of them lost with bf16.
+        fp32 values on the tensor cores are pairs of tf32 numbers: what a product loses is 2^-20 of it (two remainders cut at 2^-21).
         Then one rounding."""
         group = self.heads // self.kv_heads
         out, lse = self.out.get().double(), self.lse.get().double()
@@ -64,7 +65,7 @@ class Case:
             for h in range(self.kv_heads):
                 mine = slice(h * group, (h + 1) * group)
                 o, l, p, terms, size = attend(self.q[b, mine], k[:n, h], v[:n, h], self.scale, begin)
-                logit = (self.dim + 16) * 2.0 ** -23 * (terms + 1)
+                logit = (self.dim + 16) * 2.0 ** -23 * (terms + 1) + (2.0 ** -20 * terms if self.name == "f32" else 0)
                 rel = 2 * logit + (n / 4 + 150) * 2.0 ** -23 + (2.0 ** -16 if self.name == "bf16" else 2.0 ** -20)
                 assert ((out[b, mine] - o).abs() <= size * rel + o.abs() * HALF[self.name] + TINY[self.name] + 1e-30).all()
                 if n == 0:
@@ -131,9 +132,9 @@ def test_ragged_batches(ctx, name, batch):
     Case(ctx, name, lengths, 2, 1, 64, 16, seed=batch, weights=False).run().check()
 
 
-@pytest.mark.parametrize("name", ["f16", "bf16"])
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
 def test_on_cuda_cores(ctx, name):
-    """The kernel of fp32 and odd rows serves 16-bit types too ("tensor_cores" 0)."""
+    """The kernel of odd rows serves every row ("tensor_cores" 0)."""
     ctx.set_option("tensor_cores", 0)
     try:
         Case(ctx, name, [0, 1, 100, 1000], 10, 2, 128, 16, seed=3).run().check()
@@ -181,6 +182,23 @@ def test_rows_without_a_finite_logit(ctx, name):
     c.run()
     assert (c.out.get() == 0).all() and (c.lse.get() == -math.inf).all()
     assert np.array_equal(c.w_out.get().numpy()[..., :40], c.w_in[..., :40])
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_single_infinite_keys(ctx, name):
+    """A key that is -inf along positive queries leaves its slot without weight; the other slots share theirs as if it were not there."""
+    c = Case(ctx, name, [100], 4, 2, 64, 16, seed=5, weights=False)
+    c.q = c.q.abs() + 0.5
+    c.dq = Values(c.ctx, c.q)
+    pool = c.dk.get()
+    gone = [3, 17, 40, 99]
+    for j in gone:
+        pool[int(c.table[0, j // 16]), :, j % 16, 7] = -math.inf
+    c.dk = Values(c.ctx, pool)
+    c.run()
+    stay = [j for j in range(100) if j not in gone]
+    c.rows = [tuple(r[stay] for r in c.rows[0])]
+    c.check([len(stay)])
 
 
 def test_nan_in_a_used_slot_stays_in_its_head(ctx):
