@@ -121,6 +121,7 @@ inline Verdict check_append(const void *q, const void *q_out, const void *k, con
                             int64_t v_token, int64_t num_pages, int64_t page_size, int dtype) {
   KV_PASS(check_heads(tokens, heads, dim, dtype));
   KV_PASS(check_heads(tokens, kv_heads, dim, dtype));
+  if ((heads + 2 * kv_heads) * dim > MOST) return unsupported("tensor too large");
   KV_PASS(check_rotary(dim, rotary, tokens, heads + 2 * kv_heads));
   KV_PASS(check_stride(q_token));
   KV_PASS(check_stride(k_token));

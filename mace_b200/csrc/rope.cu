@@ -13,81 +13,64 @@
 namespace {
 
 constexpr int THREADS = 256;
+constexpr int U = 2;          // items of a thread: with two words of 16 bytes each, 64 bytes in flight
 constexpr int TABLE = 2048;   // sines and cosines a block holds at most, beyond a single token's
 
-// One of the call's tensors: `heads` heads of every token.  The destination is rows of a tensor, or slots of a pool.
+// One of the call's tensors: queries (or all there is), which go to rows of a tensor, keys and values, which go to slots of a pool;
+// values are copied.
 struct Part {
   const void *src;
   void *dst;
   int64_t src_token, src_head, dst_token, dst_head;  // strides in elements
-  int heads;
-  int turned;    // 0: copied
-  int to_slots;  // the destination is the paged pool
 };
 
 struct RopeParams {
   Part part[3];
-  int parts;
+  int end[2];                        // heads up to which they are queries, keys
   const int32_t *positions, *slots;
   const double *freq;
   int64_t tokens;
   int per_token, tokens_per_block;   // items of a token; tokens of a block
   int per_head;                      // items of a head: first those that turn, then those that copy
-  uint32_t token_mul, token_shift, head_mul, head_shift, page_mul, page_shift;
+  uint32_t token_mul, token_shift, head_mul, head_shift, page_mul, page_shift, half_mul, half_shift;
+  int copy_two;                      // ... two words each
   int half, turning, dim, page_size, kv_heads;  // half: rotary_dim / 2; turning: items of a head that turn
-  int64_t num_pages;
+  int64_t num_pages, page_row;       // page_row: elements between the heads of a page
   float cos_factor, sin_factor;
   int *status;
 };
 
-// What an item is: with V elements to a word, items 0 .. turning - 1 of a head turn (half layout: the words at jV and half + jV;
-// interleaved: the word at jV, or with V = 1 the pair at 2j), the others copy a word behind the rotated part.
+// What an item is: with V elements to a word, items 0 .. turning - 1 of a head turn two words (half layout: those at jV and half + jV;
+// interleaved: neighbours, from 2jV on), the others copy two behind the rotated part, or one where their number is odd.
 template <typename T, int V, bool INTERLEAVED>
 struct Item {
   elem::Vec<T, V> a, b;
-  T *dst;          // of the head; null: nothing to do
-  int at, pair;    // a's place in the head; the first pair's number, or -1: copied
-  int token;       // of the block
+  int at, next, pair;       // a's place in the head, b's behind it; the first pair's number, -1: behind the rotated part
+  int token, head, which;   // of the block; of its tensor, the tensor
+  bool two;                 // there is a second word
 
-  static constexpr bool TWO = !INTERLEAVED || V == 1;   // a turning item has two words
-
+  // Where it comes from, and the loads.  (Where it goes needs the tokens' slots: those are read in the meantime.)
   __device__ __forceinline__ void fetch(const RopeParams &p, int64_t token0, int tokens, int index) {
-    dst = nullptr;
     token = p.tokens_per_block == 1 ? 0 : static_cast<int>(fast_div(index, p.token_mul, p.token_shift));
     const int rest = index - token * p.per_token;
+    which = -1;
     if (token >= tokens || rest >= p.per_token) return;
-    int head = static_cast<int>(fast_div(rest, p.head_mul, p.head_shift));
+    head = static_cast<int>(fast_div(rest, p.head_mul, p.head_shift));
     const int j = rest - head * p.per_head;
-    int which = 0;
-    while (which + 1 < p.parts && head >= p.part[which].heads) head -= p.part[which++].heads;
+    which = (head >= p.end[0]) + (head >= p.end[1]);
+    head -= which == 0 ? 0 : which == 1 ? p.end[0] : p.end[1];
     const Part &part = p.part[which];
     const T *src = static_cast<const T *>(part.src) + (token0 + token) * part.src_token + head * part.src_head;
     const bool turns = j < p.turning;
-    if (turns) {
-      at = INTERLEAVED && V == 1 ? 2 * j : j * V;
-      pair = !part.turned ? -1 : INTERLEAVED && V > 1 ? j * (V / 2) : j * V;
-    } else {
-      at = 2 * p.half + (j - p.turning) * V;
-      pair = -2;
-    }
-    if (part.to_slots) {
-      const int slot = mb_load(p.slots + token0 + token);
-      if (slot < 0) return;
-      const int page = static_cast<int>(fast_div(slot, p.page_mul, p.page_shift));
-      const int64_t to = kv::row_offset(page, p.num_pages, p.kv_heads, head, p.page_size, slot - page * p.page_size, p.dim);
-      if (to < 0) {
-        mb_report_bad_index(p.status);
-        return;
-      }
-      dst = static_cast<T *>(part.dst) + to;
-    } else {
-      dst = static_cast<T *>(part.dst) + (token0 + token) * part.dst_token + head * part.dst_head;
-    }
+    at = turns ? (INTERLEAVED ? 2 * j * V : j * V) : 2 * p.half + (j - p.turning) * (p.copy_two ? 2 * V : V);
+    pair = turns ? j * V : -1;
+    two = turns || p.copy_two;
+    next = !turns ? V : INTERLEAVED ? V : p.half;
     a.load(src + at);
-    if (TWO && turns) b.load(src + other(p));
+    if (two) b.load(src + at + next);
   }
 
-  static constexpr int PAIRS = TWO ? V : V / 2;         // that a turning item has
+  static constexpr int PAIRS = V;   // that a turning item has
 
   // Where pair q of a token lies in its table: two of an item's side by side, words of neighbouring items next to each other, so that
   // lanes read 16 bytes each without meeting in a bank.
@@ -97,11 +80,19 @@ struct Item {
     return ((i / 2) * items + j) * 2 + i % 2;
   }
 
-  __device__ __forceinline__ int other(const RopeParams &p) const { return INTERLEAVED ? at + 1 : at + p.half; }
-
-  __device__ __forceinline__ void finish(const RopeParams &p, const float2 *table) {
-    if (dst == nullptr) return;
-    if (pair >= 0) {
+  __device__ __forceinline__ void finish(const RopeParams &p, int64_t token0, const float2 *table, const int64_t *rows) {
+    if (which < 0) return;
+    const Part &part = p.part[which];
+    int64_t to;
+    if (which == 0) {
+      to = (token0 + token) * part.dst_token + head * part.dst_head;
+    } else {
+      to = rows[token];
+      if (to < 0) return;
+      to += head * p.page_row;
+    }
+    T *dst = static_cast<T *>(part.dst) + to;
+    if (pair >= 0 && which != 2) {
       float2 cs[PAIRS];
       if constexpr (PAIRS == 1) {
         cs[0] = table[token * p.half + pair];
@@ -115,21 +106,22 @@ struct Item {
       }
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {
-        T &lo = TWO ? a.v[i] : a.v[(2 * i) % V], &hi = TWO ? b.v[i] : a.v[(2 * i + 1) % V];
+        // half layout (and single values): a's i-th and b's; interleaved: two neighbours, of a, then of b
+        constexpr bool APART = !INTERLEAVED || V == 1;
+        elem::Vec<T, V> &first = APART || i < V / 2 ? a : b, &second = APART || i >= V / 2 ? b : a;
+        T &lo = first.v[APART ? i : 2 * i % V], &hi = second.v[APART ? i : (2 * i + 1) % V];
         const float x = elem::widen(lo), y = elem::widen(hi), c = cs[i].x, s = cs[i].y;
         lo = elem::narrow<T>(x * c - y * s);
         hi = elem::narrow<T>(x * s + y * c);
       }
     }
     a.store(dst + at);
-    if (TWO && pair != -2) b.store(dst + other(p));
+    if (two) b.store(dst + at + next);
   }
 };
 
 template <typename T, int V, bool INTERLEAVED>
 __global__ void __launch_bounds__(THREADS) rope_kernel(const RopeParams p) {
-  // two words per item: two items a thread; else four.  64 bytes of a thread's are in flight.
-  constexpr int U = Item<T, V, INTERLEAVED>::TWO ? 2 : 4;
   extern __shared__ __align__(16) float2 table[];
   mb_grid_dep_launch();
   mb_grid_dep_wait();
@@ -138,8 +130,21 @@ __global__ void __launch_bounds__(THREADS) rope_kernel(const RopeParams p) {
   Item<T, V, INTERLEAVED> item[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) item[u].fetch(p, token0, tokens, (blockIdx.y * U + u) * THREADS + threadIdx.x);
+  int64_t *rows = reinterpret_cast<int64_t *>(table + tokens * p.half);   // where the tokens' first heads go in the pools, -1: nowhere
+  if (p.slots != nullptr) {
+    for (int i = THREADS - 1 - threadIdx.x; i < tokens; i += THREADS) {   // (from the last warp down: the first ones have the table)
+      const int slot = mb_load(p.slots + token0 + i);
+      int64_t to = -1;
+      if (slot >= 0) {
+        const int page = static_cast<int>(fast_div(slot, p.page_mul, p.page_shift));
+        to = kv::row_offset(page, p.num_pages, p.kv_heads, 0, p.page_size, slot - page * p.page_size, p.dim);
+        if (to < 0) mb_report_bad_index(p.status);
+      }
+      rows[i] = to;
+    }
+  }
   for (int i = threadIdx.x; i < tokens * p.half; i += THREADS) {
-    const int token = i / p.half;
+    const int token = tokens == 1 ? 0 : static_cast<int>(fast_div(i, p.half_mul, p.half_shift));
     const double turns = mb_load(p.positions + token0 + token) * (mb_load(p.freq + (i - token * p.half)) * 0.15915494309189533577);
     float s, c;
     sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &c);
@@ -147,14 +152,15 @@ __global__ void __launch_bounds__(THREADS) rope_kernel(const RopeParams p) {
   }
   __syncthreads();
 #pragma unroll
-  for (int u = 0; u < U; ++u) item[u].finish(p, table);
+  for (int u = 0; u < U; ++u) item[u].finish(p, token0, table, rows);
 }
 
 template <typename T, int V, bool INTERLEAVED>
 int launch(mb_context *ctx, RopeParams &p, int heads) {
-  constexpr int U = Item<T, V, INTERLEAVED>::TWO ? 2 : 4;
-  p.turning = INTERLEAVED && V > 1 ? 2 * p.half / V : p.half / V;
-  p.per_head = p.turning + (p.dim - 2 * p.half) / V;
+  const int behind = (p.dim - 2 * p.half) / V;
+  p.turning = p.half / V;
+  p.copy_two = behind % 2 == 0;
+  p.per_head = p.turning + (p.copy_two ? behind / 2 : behind);
   if (p.per_head > INT32_MAX / heads) return mb_fail(ctx, MB_UNSUPPORTED, "mb_rope: a token has too many values");
   p.per_token = p.per_head * heads;
   int64_t tokens = std::min<int64_t>(U * THREADS / p.per_token, p.tokens);
@@ -167,7 +173,8 @@ int launch(mb_context *ctx, RopeParams &p, int heads) {
   const int64_t blocks = ceil_div64(p.tokens, p.tokens_per_block);
   const int64_t rows = ceil_div64(static_cast<int64_t>(p.per_token) * p.tokens_per_block, U * THREADS);
   if (rows > 65535) return mb_fail(ctx, MB_UNSUPPORTED, "mb_rope: a token has too many values");
-  const size_t smem = sizeof(float2) * p.tokens_per_block * p.half;
+  fast_div_make(p.half, &p.half_mul, &p.half_shift);
+  const size_t smem = (sizeof(float2) * p.half + (p.slots != nullptr ? sizeof(int64_t) : 0)) * p.tokens_per_block;
   if (smem > (48u << 10)) return mb_fail(ctx, MB_UNSUPPORTED, "mb_rope: rotary_dim above 12288");
   MB_CUDA(ctx, mb_launch_chained(ctx, rope_kernel<T, V, INTERLEAVED>, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(rows)),
                                  dim3(THREADS), smem, p));
@@ -177,22 +184,21 @@ int launch(mb_context *ctx, RopeParams &p, int heads) {
 
 // The widest word that every row and place allows: 16 bytes, two elements, or one.
 template <typename T>
-int dispatch(mb_context *ctx, RopeParams &p, bool interleaved) {
-  int heads = 0;
+int dispatch(mb_context *ctx, RopeParams &p, bool interleaved, int heads) {
+  const int parts = p.slots != nullptr ? 3 : 1;
   bool words[2] = {true, true};
   constexpr int wide = 16 / sizeof(T);
   const int sizes[2] = {wide, 2};
   for (int i = 0; i < 2; ++i) {
     const int v = sizes[i], behind = p.dim - 2 * p.half;
-    words[i] = behind % v == 0 && (interleaved ? 2 * p.half : p.half) % v == 0;
-    for (int w = 0; w < p.parts; ++w) {
+    words[i] = behind % v == 0 && p.half % v == 0;
+    for (int w = 0; w < parts; ++w) {
       const Part &part = p.part[w];
       words[i] = words[i] && kv::aligned(part.src, v * sizeof(T)) && kv::aligned(part.dst, v * sizeof(T)) &&
                  part.src_token % v == 0 && part.src_head % v == 0 && part.dst_token % v == 0 && part.dst_head % v == 0 &&
-                 (!part.to_slots || p.dim % v == 0);
+                 (w == 0 || p.dim % v == 0);
     }
   }
-  for (int w = 0; w < p.parts; ++w) heads += p.part[w].heads;
   if (interleaved) {
     if (words[0]) return launch<T, wide, true>(ctx, p, heads);
     if (words[1]) return launch<T, 2, true>(ctx, p, heads);
@@ -258,14 +264,14 @@ int mb_rope(mb_context *ctx, const void *x, void *y, const int32_t *positions, c
   if (tokens == 0) return MB_SUCCESS;
   MB_CUDA(ctx, cudaSetDevice(ctx->device));
   RopeParams p = {};
-  p.part[0] = {x, y, x_token_stride, x_head_stride, y_token_stride, y_head_stride, static_cast<int>(heads), 1, 0};
-  p.parts = 1;
+  p.part[0] = {x, y, x_token_stride, x_head_stride, y_token_stride, y_head_stride};
+  p.end[0] = p.end[1] = static_cast<int>(heads);
   p.positions = positions; p.freq = freq; p.tokens = tokens;
   p.half = static_cast<int>(rotary_dim / 2); p.dim = static_cast<int>(head_dim);
   p.cos_factor = magnitude; p.sin_factor = inverse ? -magnitude : magnitude;
   p.status = ctx->dev_status;
   int st = MB_SUCCESS;
-  MB_FOR_ELEMENT(dtype, st = dispatch<T>(ctx, p, interleaved != 0));
+  MB_FOR_ELEMENT(dtype, st = dispatch<T>(ctx, p, interleaved != 0, static_cast<int>(heads)));
   return st;
 }
 
@@ -283,10 +289,11 @@ int mb_rope_kv_append(mb_context *ctx, const void *q, void *q_out, const void *k
   MB_CUDA(ctx, cudaSetDevice(ctx->device));
   RopeParams p = {};
   const int h = static_cast<int>(heads), hk = static_cast<int>(kv_heads);
-  p.part[0] = {q, q_out, q_token_stride, head_dim, q_out_token_stride, head_dim, h, 1, 0};
-  p.part[1] = {k, k_cache, k_token_stride, head_dim, 0, 0, hk, 1, 1};
-  p.part[2] = {v, v_cache, v_token_stride, head_dim, 0, 0, hk, 0, 1};
-  p.parts = 3;
+  p.part[0] = {q, q_out, q_token_stride, head_dim, q_out_token_stride, head_dim};
+  p.part[1] = {k, k_cache, k_token_stride, head_dim, 0, 0};
+  p.part[2] = {v, v_cache, v_token_stride, head_dim, 0, 0};
+  p.end[0] = h; p.end[1] = h + hk;
+  p.page_row = page_size * head_dim;
   p.positions = positions; p.slots = slots; p.freq = freq; p.tokens = tokens;
   p.half = static_cast<int>(rotary_dim / 2); p.dim = static_cast<int>(head_dim);
   p.num_pages = num_pages; p.page_size = static_cast<int>(page_size); p.kv_heads = hk;
@@ -294,7 +301,7 @@ int mb_rope_kv_append(mb_context *ctx, const void *q, void *q_out, const void *k
   p.cos_factor = p.sin_factor = magnitude;
   p.status = ctx->dev_status;
   int st = MB_SUCCESS;
-  MB_FOR_ELEMENT(dtype, st = dispatch<T>(ctx, p, interleaved != 0));
+  MB_FOR_ELEMENT(dtype, st = dispatch<T>(ctx, p, interleaved != 0, h + 2 * hk));
   return st;
 }
 
