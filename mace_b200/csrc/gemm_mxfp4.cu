@@ -311,15 +311,22 @@ gemm_mxfp4_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     const int tn = first % p.tiles_n, tm = first / p.tiles_n;
     const int rows = min(BT, p.M - tm * BT);
     const uint32_t mine = smem_u32(smem);
-    for (int i = rank * TC_THREADS + threadIdx.x; i < rows * 128; i += p.splits * TC_THREADS) {
-      const int64_t n = static_cast<int64_t>(tn) * 128 + i % 128, m = static_cast<int64_t>(tm) * BT + i / 128;
-      float sum = 0.f;
+    // four neighbouring n at a time
+    for (int i = rank * TC_THREADS + threadIdx.x; i < rows * 32; i += p.splits * TC_THREADS) {
+      const int64_t n = static_cast<int64_t>(tn) * 128 + i % 32 * 4, m = static_cast<int64_t>(tm) * BT + i / 32;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
       for (int s = 0; s < p.splits; ++s) {
-        float v;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(mine + 4 * i, s)) : "memory");
-        sum += v;
+        float v[4];
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(mapa_shared(mine + 16 * i, s)) : "memory");
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] += v[j];
       }
-      if (n < p.N) static_cast<T *>(p.c)[m * p.stride + n] = elem::narrow<T>(sum);
+      T *to = static_cast<T *>(p.c) + m * p.stride + n;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n + j < p.N) to[j] = elem::narrow<T>(sum[j]);
     }
     // no CTA of a cluster may leave while another still reads its tile
     cluster_sync_all();
@@ -356,14 +363,25 @@ int launch_tc(mb_context *ctx, MxGemmParams &p, int splits, int type) {
 
 template <typename T>
 int gemm_tc(mb_context *ctx, MxGemmParams &p, int type) {
-  // few tokens: one tile of them, the depth over a cluster as far as there are SMs and steps; else CTAs that walk over tiles
+  // The tile width and cut with the smallest estimate, in nanoseconds.  Measured: a step's bytes come at 88 a nanosecond with every SM
+  // asking; around a CTA's steps 3.5 us for a first round, 0.6 for a further one; joining a cluster's parts 0.8 us and 8 ns a token.
+  // 4096 x 4096 weights: 1 token 5.8 us (16 x 4 CTAs a tile), 128 8.3, 512 9.8 (128 wide, uncut), 1000 11.4 (256 wide, uncut; 128 wide, two
+  // rounds: 16.1).
   const int64_t steps = (p.blocks + 7) / 8;
-  const int64_t columns = p.M <= 16 ? 16 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : p.M <= 128 ? 128 : 256;
-  int bt = static_cast<int>(columns);
-  if (bt == 256 && p.tiles_n * ceil_div64(p.M, 256) < ctx->num_sms) bt = 128;
-  const int64_t tiles = p.tiles_n * ceil_div64(p.M, bt);
-  int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= mb_resident_cluster_ctas(ctx, splits * 2) && splits * 2 <= steps) splits *= 2;
+  int bt = 256, splits = 1;
+  int64_t best = -1;
+  for (const int w : {16, 32, 64, 128, 256}) {
+    if (w < 128 && p.M > w) continue;   // (narrower tiles than a tile of scales: one of them only)
+    if (w > 16 && p.M <= w / 2) break;
+    const int64_t tiles = p.tiles_n * ceil_div64(p.M, w);
+    const int64_t step = (128 * 128 + w * 128 + 1024 + (w + 127) / 128 * 1024) / 88;
+    for (const int s : {1, 2, 4, 8}) {
+      if (s > steps) break;
+      const int64_t rounds = ceil_div64(tiles * s, mb_resident_cluster_ctas(ctx, s));
+      const int64_t cost = 3500 + (rounds - 1) * 600 + rounds * ceil_div64(steps, s) * step + (s > 1 ? rounds * (800 + 8 * w) : 0);
+      if (best < 0 || cost < best) best = cost, bt = w, splits = s;
+    }
+  }
   switch (bt) {
     case 16: return launch_tc<T, 16>(ctx, p, splits, type);
     case 32: return launch_tc<T, 32>(ctx, p, splits, type);
