@@ -557,9 +557,10 @@ template <> struct Mma<float> {
     asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
-  // x as a tf32 number and what that leaves, whose own tf32 part ends at 2^-21 of x (of an infinity: NaN)
+  // x as the nearest tf32 number and what that leaves, 12 bits, of which the MMA takes 11: together x to 2^-23 (of an infinity, or of a
+  // number that has none above it: NaN)
   static __device__ __forceinline__ void split(uint32_t x, uint32_t &hi, uint32_t &lo) {
-    hi = x & 0xffffe000u;
+    hi = (x + 0x1000u) & 0xffffe000u;
     lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
   }
 };
@@ -730,6 +731,8 @@ __global__ void __launch_bounds__(THREADS) paged_attention_mma_kernel(const Atte
     for (int t = 0; t < HEADS; ++t)
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[t][j] = 0.f;
+    // (fp32: an MMA cuts its sum off, always towards zero; so large products gather in fours, small ones by themselves)
+    float large[4] = {0.f, 0.f, 0.f, 0.f}, small[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int d = 0; d < STEPS; ++d) {
       uint32_t a[4];
@@ -740,9 +743,16 @@ __global__ void __launch_bounds__(THREADS) paged_attention_mma_kernel(const Atte
         for (int i = 0; i < 4; ++i) Mma<T>::split(a[i], hi[i], lo[i]);
 #pragma unroll
         for (int i = 0; i < 2; ++i) Mma<T>::split(q[0][d][i], qh[i], ql[i]);
-        Mma<T>::run(s[0], hi, ql[0], ql[1]);
-        Mma<T>::run(s[0], lo, qh[0], qh[1]);
-        Mma<T>::run(s[0], hi, qh[0], qh[1]);
+        Mma<T>::run(small, hi, ql[0], ql[1]);
+        Mma<T>::run(small, lo, qh[0], qh[1]);
+        Mma<T>::run(large, hi, qh[0], qh[1]);
+        if (d % 4 == 3) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            s[0][j] += d == STEPS - 1 ? large[j] + small[j] : large[j];
+            large[j] = 0.f;
+          }
+        }
       } else {
 #pragma unroll
         for (int t = 0; t < HEADS; ++t) Mma<T>::run(s[t], a, q[t][d][0], q[t][d][1]);
@@ -827,26 +837,33 @@ __global__ void __launch_bounds__(THREADS) paged_attention_mma_kernel(const Atte
         *reinterpret_cast<float2 *>(&weight_s[warp][row + 8 * i][2 * pair]) = make_float2(x, y);
       }
       __syncwarp();
+      uint32_t ph[4], pl[4];   // slots pair, pair + 4 of the first eight, of the others
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {   // eight slots
-        uint32_t ph[2], pl[2];
+      for (int i = 0; i < 4; ++i) Mma<T>::split(__float_as_uint(weight_s[warp][i * 4 + pair][row]), ph[i], pl[i]);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) Mma<T>::split(__float_as_uint(weight_s[warp][half * 8 + i * 4 + pair][row]), ph[i], pl[i]);
+      for (int d = 0; d < DIM_STEPS; ++d) {
+        uint32_t hi[2][4], lo[2][4];
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int d = 0; d < DIM_STEPS; ++d) {
-          uint32_t hi[4], lo[4];
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             // (the swizzle's low three bits: every other 16 values are four words on)
             const uint32_t addr = values + half * 8 * G::ROW + ((value_word[i] ^ (d % 2 << 6)) + d / 2 * 128);
             uint32_t x;
             asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(addr) : "memory");
-            Mma<T>::split(x, hi[i], lo[i]);
+            Mma<T>::split(x, hi[half][i], lo[half][i]);
           }
-          Mma<T>::run(acc[0][d], hi, pl[0], pl[1]);
-          Mma<T>::run(acc[0][d], lo, ph[0], ph[1]);
-          Mma<T>::run(acc[0][d], hi, ph[0], ph[1]);
+        // small products first; what the chunk gives is added to the sum by rounding
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          Mma<T>::run(part, hi[half], pl[2 * half], pl[2 * half + 1]);
+          Mma<T>::run(part, lo[half], ph[2 * half], ph[2 * half + 1]);
         }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) Mma<T>::run(part, hi[half], ph[2 * half], ph[2 * half + 1]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[0][d][j] += part[j];
       }
       __syncwarp();
     } else {
