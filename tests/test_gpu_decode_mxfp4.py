@@ -150,7 +150,7 @@ def _check(got, a, b, bias, name, cores=False):
 
 SHAPES = [(1, 1, 1), (1, 16, 32), (1, 4096, 4096), (3, 130, 100), (16, 333, 777), (17, 128, 64), (128, 128, 128), (129, 127, 300), (200, 1000, 513),
           (64, 4099, 256), (513, 640, 1024), (40, 8192, 160), (300, 260, 4096), (1000, 1000, 96),
-          (2500, 2100, 160), (2563, 2305, 700), (4097, 1280, 64)]
+          (2500, 2100, 160), (2563, 2305, 700), (4097, 1280, 64), (5000, 2300, 4128), (3000, 4224, 2080)]
 
 
 @pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
