@@ -12,10 +12,8 @@
 
 namespace {
 
-constexpr int SELECT_THREADS = 512;
-constexpr int SELECT_WARPS = SELECT_THREADS / 32;
 constexpr int COPY_THREADS = 256;
-constexpr int COPY_EACH = 4;   // words a thread has in flight, of keys and of values each
+constexpr int COPY_EACH = 2;   // words a thread has in flight, of keys and of values each (four: 57.9 us for 54.5 at 16 x 8 heads of 2048 kept)
 
 struct EvictParams {
   const void *k_src, *v_src;
@@ -49,7 +47,7 @@ __device__ __forceinline__ unsigned load_remote_u32(uint32_t addr, int rank) {
 // A cluster of CTAs per sequence and kv head, each with a run of the candidates, whose order-preserving integers it keeps in shared
 // memory (where they fit: `cached`).  Digits of 11, 11 and 10 bits; every CTA counts its own, after a cluster barrier each adds up all
 // CTAs' counts through distributed shared memory and comes to the same digit.  What bounds it: two passes over counts and a cluster
-// barrier for each digit, about 1 us, not the weights (33333 of them, 4 heads: 39 us with one CTA a head and bytes as digits, SELECT_US here).
+// barrier for each digit, about 1 us, not the weights (33333 of them, 4 heads: 39 us with one CTA a head and bytes as digits, 18 here).
 constexpr int DIGIT = 2048, GROUPS = DIGIT / 32;
 
 // The sum over the lanes up to this one.
@@ -62,7 +60,9 @@ __device__ __forceinline__ unsigned upto_lane(unsigned v, int lane) {
   return v;
 }
 
-__global__ void __launch_bounds__(SELECT_THREADS, 2) evict_select_kernel(const EvictParams p) {
+template <int SELECT_THREADS>
+__global__ void __launch_bounds__(SELECT_THREADS, 1024 / SELECT_THREADS) evict_select_kernel(const EvictParams p) {
+  constexpr int SELECT_WARPS = SELECT_THREADS / 32;
   extern __shared__ uint32_t keys[];
   __shared__ __align__(8) unsigned counts[3][DIGIT], groups[3][GROUPS];
   __shared__ unsigned above[SELECT_WARPS], equal[SELECT_WARPS], mine[2];
@@ -111,18 +111,21 @@ __global__ void __launch_bounds__(SELECT_THREADS, 2) evict_select_kernel(const E
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
       const uint32_t digits = pass == 2 ? 1023u : 2047u;
       unsigned *count = counts[pass];
+#pragma unroll 4
       for (int base = from; base < until; base += SELECT_THREADS) {
         const int j = base + t;
         const uint32_t u = j < until ? key(j) : 0;
         const bool counts_in = j < until && (u & mask) == prefix;
+        const unsigned in = __ballot_sync(0xffffffffu, counts_in);
+        if (in == 0) continue;
         const uint32_t d = (u >> shift) & digits;
         // (weights that are all alike would queue at one counter)
-        int same;
-        __match_all_sync(0xffffffffu, counts_in ? d : 0xffffffffu, &same);
-        if (!same) {
-          if (counts_in) atomicAdd(count + d, 1u);
-        } else if (counts_in && lane == 0) {
-          atomicAdd(count + d, 32u);
+        int same = 0;
+        if (in == 0xffffffffu) __match_all_sync(0xffffffffu, d, &same);
+        if (same) {
+          if (lane == 0) atomicAdd(count + d, 32u);
+        } else if (counts_in) {
+          atomicAdd(count + d, 1u);
         }
       }
       __syncthreads();
@@ -219,6 +222,8 @@ __global__ void __launch_bounds__(SELECT_THREADS, 2) evict_select_kernel(const E
       a += load_remote_u32(sm100::smem_u32(&mine[0]), s);
       e += load_remote_u32(sm100::smem_u32(&mine[1]), s);
     }
+    // (no CTA may leave while another reads its counts: arrive here, wait at the end)
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   }
   for (int base = mine_from; base < mine_until; base += 32) {
     const int j = base + lane;
@@ -232,7 +237,7 @@ __global__ void __launch_bounds__(SELECT_THREADS, 2) evict_select_kernel(const E
     a += __popc(more);
     e += __popc(same);
   }
-  if (p.cluster > 1) sm100::cluster_sync_all();   // (no CTA may leave while another reads its counts)
+  if (p.cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // Rows of keys and values to their new slots, a word per item, their weights, and the new lengths (here, because the other kernel reads the old ones
@@ -344,21 +349,25 @@ extern "C" int mb_kv_evict(mb_context *ctx, const void *k_src, const void *v_src
                          reinterpret_cast<uintptr_t>(v_dst) | static_cast<uintptr_t>(row_bytes);
   if (row_bytes / (bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 2) > COPY_THREADS * COPY_EACH)
     return mb_fail(ctx, MB_UNSUPPORTED, "mb_kv_evict: head_dim too large");
-  // two CTAs an SM, and 2048 weights or more to each
-  constexpr int MOST_KEYS = 20 << 10;   // (two CTAs' runs fit)
+  // A CTA of 1024 threads an SM, or, where there are more heads than SMs, two of 512; 4096 weights or more to each of a cluster.
+  // (16 sequences of 8192, 8 heads: two CTAs of 512 a head 17.7 us, one of 1024 14.7.)
+  constexpr int MOST_KEYS = 20 << 10;
+  const bool large = units <= ctx->num_sms;
   p.cluster = 1;
-  while (p.cluster < 16 && units * p.cluster * 2 <= 2 * ctx->num_sms && p.longest > 2048 * p.cluster) p.cluster *= 2;
+  while (p.cluster < 16 && units * p.cluster * 2 <= ctx->num_sms && p.longest > 4096 * p.cluster) p.cluster *= 2;
   while (p.cluster < 16 && p.longest > MOST_KEYS * p.cluster) p.cluster *= 2;
   const int64_t keys = ceil_div64(p.longest, p.cluster);
   p.cached = keys <= MOST_KEYS;
   if (units * p.cluster > kv::MOST) return mb_fail(ctx, MB_UNSUPPORTED, "mb_kv_evict: too many kv heads");
   if (!ctx->evict_attr_set) {
-    MB_CUDA(ctx, cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_KEYS * 4));
-    MB_CUDA(ctx, cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));   // clusters of 16
+    for (const auto kern : {evict_select_kernel<512>, evict_select_kernel<1024>}) {
+      MB_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_KEYS * 4));
+      MB_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));   // clusters of 16
+    }
     ctx->evict_attr_set = true;
   }
-  MB_CUDA(ctx, mb_launch_clusters(ctx, evict_select_kernel, static_cast<unsigned>(units * p.cluster), SELECT_THREADS,
-                                  p.cached ? static_cast<size_t>(keys) * 4 : 0, p.cluster, p));
+  MB_CUDA(ctx, mb_launch_clusters(ctx, large ? evict_select_kernel<1024> : evict_select_kernel<512>, static_cast<unsigned>(units * p.cluster),
+                                  large ? 1024 : 512, p.cached ? static_cast<size_t>(keys) * 4 : 0, p.cluster, p));
   ctx->launches++;
   if (bits % 16 == 0) return launch_copy<uint4>(ctx, p, units, row_bytes);
   if (bits % 4 == 0) return launch_copy<uint32_t>(ctx, p, units, row_bytes);
