@@ -30,12 +30,13 @@ struct MxParams {
 template <typename T>
 struct Eight {
   uint32_t word[EACH * sizeof(T) / 4];
-  __device__ __forceinline__ void load(const MxParams &p, const T *row, int col) {
+  // left: values of the row from here on
+  __device__ __forceinline__ void load(const T *from, int left, bool vec) {
     constexpr int WORDS = sizeof(word) / 16;
-    if (p.vec && col + EACH <= p.cols) {
+    if (vec && left >= EACH) {
 #pragma unroll
       for (int w = 0; w < WORDS; ++w) {
-        const uint4 v = mb_load(reinterpret_cast<const uint4 *>(row + col) + w);
+        const uint4 v = mb_load(reinterpret_cast<const uint4 *>(from) + w);
         word[4 * w] = v.x, word[4 * w + 1] = v.y, word[4 * w + 2] = v.z, word[4 * w + 3] = v.w;
       }
     } else {
@@ -45,8 +46,8 @@ struct Eight {
         pack.word = 0;
 #pragma unroll
         for (int i = 0; i < static_cast<int>(4 / sizeof(T)); ++i) {
-          const int at = col + w * (4 / sizeof(T)) + i;
-          if (at < p.cols) pack.v[i] = mb_load(row + at);
+          const int at = w * (4 / sizeof(T)) + i;
+          if (at < left) pack.v[i] = mb_load(from + at);
         }
         word[w] = pack.word;
       }
@@ -115,6 +116,19 @@ struct Span {
   }
   __device__ __forceinline__ int64_t row_of(const MxParams &p, int i) const { return WIDE ? row : row + i * p.block_rows; }
   __device__ __forceinline__ int chunk_of(int i) const { return WIDE ? chunk + i * THREADS : chunk; }
+  // Addresses of group i: with WIDE a constant behind the first one's.
+  template <typename P>
+  __device__ __forceinline__ P *values(const MxParams &p, P *first, int i) const {
+    return WIDE ? first + i * THREADS * EACH : first + i * p.block_rows * p.stride;
+  }
+  __device__ __forceinline__ uint32_t *codes(const MxParams &p, uint32_t *first, int blocks, int i) const {
+    return WIDE ? first + i * THREADS : first + static_cast<int64_t>(i) * p.block_rows * blocks * 4;
+  }
+  __device__ __forceinline__ uint8_t *scales(const MxParams &p, uint8_t *first, int i) const {
+    static_assert(THREADS * EACH % (mx::BLOCK * mx::TILE_BLOCKS) == 0, "whole tiles");
+    return WIDE ? first + i * (THREADS * EACH / (mx::BLOCK * mx::TILE_BLOCKS)) * mx::TILE_BYTES
+                : p.scales + mx::scale_at(row_of(p, i), chunk / (mx::BLOCK / EACH), p.tiles);
+  }
 };
 
 // Items are (row, group of eight) of the whole tiles: a lane whose block does not exist writes the tile's zeros.  Rows are whole groups
@@ -126,14 +140,16 @@ __global__ void __launch_bounds__(THREADS) quantize_mxfp4_kernel(const MxParams 
   const Span<WIDE> at(p);
   const int blocks = static_cast<int>(mx::blocks_of(p.cols));
   const int64_t tile_rows = mx::tile_rows(p.rows) * mx::TILE_ROWS;
+  const T *x0 = static_cast<const T *>(p.x) + at.row * p.stride + at.chunk * EACH;
+  uint32_t *codes0 = reinterpret_cast<uint32_t *>(p.codes) + at.row * blocks * 4 + at.chunk;
+  uint8_t *scales0 = p.scales + mx::scale_at(at.row, at.chunk / (mx::BLOCK / EACH), p.tiles);
   Eight<T> x[TIMES];
 #pragma unroll
   for (int i = 0; i < TIMES; ++i) {
-    const int64_t row = at.row_of(p, i);
-    const int col = at.chunk_of(i) * EACH;
+    const int left = p.cols - at.chunk_of(i) * EACH;
 #pragma unroll
     for (uint32_t &w : x[i].word) w = 0;
-    if (row < p.rows && col < p.cols) x[i].load(p, static_cast<const T *>(p.x) + row * p.stride, col);
+    if (at.row_of(p, i) < p.rows && left > 0) x[i].load(at.values(p, x0, i), left, p.vec);
   }
 #pragma unroll
   for (int i = 0; i < TIMES; ++i) {
@@ -156,9 +172,9 @@ __global__ void __launch_bounds__(THREADS) quantize_mxfp4_kernel(const MxParams 
     uint32_t four = there ? scale : 0;
     four |= __shfl_down_sync(0xffffffffu, four, 4, 16) << 8;
     four |= __shfl_down_sync(0xffffffffu, four, 8, 16) << 16;
-    if (there) reinterpret_cast<uint32_t *>(p.codes + row * blocks * 16)[chunk] = word;
+    if (there) *at.codes(p, codes0, blocks, i) = word;
     if ((threadIdx.x & 15) == 0 && row < tile_rows && chunk < p.chunks)
-      *reinterpret_cast<uint32_t *>(p.scales + mx::scale_at(row, block, p.tiles)) = four;
+      *reinterpret_cast<uint32_t *>(at.scales(p, scales0, i)) = four;
   }
 }
 
@@ -168,6 +184,9 @@ __global__ void __launch_bounds__(THREADS) dequantize_mxfp4_kernel(const MxParam
   mb_grid_dep_wait();
   const Span<WIDE> at(p);
   const int blocks = static_cast<int>(mx::blocks_of(p.cols));
+  T *y0 = static_cast<T *>(p.y) + at.row * p.stride + at.chunk * EACH;
+  uint32_t *codes0 = reinterpret_cast<uint32_t *>(p.codes) + at.row * blocks * 4 + at.chunk;
+  uint8_t *scales0 = p.scales + mx::scale_at(at.row, at.chunk / (mx::BLOCK / EACH), p.tiles);
   uint32_t word[TIMES];
   int scale[TIMES];
 #pragma unroll
@@ -176,8 +195,8 @@ __global__ void __launch_bounds__(THREADS) dequantize_mxfp4_kernel(const MxParam
     const int chunk = at.chunk_of(i);
     word[i] = scale[i] = 0;
     if (row < p.rows && chunk * EACH < p.cols) {
-      word[i] = mb_load(reinterpret_cast<const uint32_t *>(p.codes + row * blocks * 16) + chunk);
-      scale[i] = mb_load(p.scales + mx::scale_at(row, chunk / (mx::BLOCK / EACH), p.tiles));
+      word[i] = mb_load(at.codes(p, codes0, blocks, i));
+      scale[i] = mb_load(at.scales(p, scales0, i));
     }
   }
 #pragma unroll
@@ -187,7 +206,7 @@ __global__ void __launch_bounds__(THREADS) dequantize_mxfp4_kernel(const MxParam
     if (row >= p.rows || col >= p.cols) continue;
     // 2^(scale - 127): scale 0 is the subnormal 2^-127, 255 is NaN
     const float unit = __uint_as_float(scale[i] == 255 ? 0x7fc00000u : scale[i] == 0 ? 0x00400000u : static_cast<uint32_t>(scale[i]) << 23);
-    T *to = static_cast<T *>(p.y) + row * p.stride + col;
+    T *to = at.values(p, y0, i);
     constexpr int W = 16 / sizeof(T);
     elem::Vec<T, W> out[EACH / W];
 #pragma unroll
