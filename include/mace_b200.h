@@ -466,8 +466,8 @@ int mb_histogram_f32(mb_context *ctx, const float *in, int64_t size, float min_v
  * cache, and eviction from that cache.
  *
  * Element types (DT_FLOAT, DT_HALF and DT_BFLOAT16 of the reference): values of
- * the 16-bit types are widened to fp32,
- * every sum is kept in fp32, results are rounded once, to nearest even.
+ * the 16-bit types are widened to fp32, every sum is kept in fp32, results are
+ * rounded once, to nearest even.
  *
  * All calls enqueue on the context's stream and may be captured into a graph
  * (mb_graph_begin; run the sequence once uncaptured first, as ever).  Indices
@@ -552,7 +552,8 @@ int mb_rope_kv_append(mb_context *ctx, const void *q, void *q_out,
  * receives weights_in[j] (0 where weights_in is NULL; weights_in ==
  * weights_out is allowed) plus the sum of p_j over the query heads that kv
  * head h serves; slots outside the window receive weights_in alone, entries
- * from lengths[b] on stay as they are.  head_dim up to 256.  An infinite
+ * from lengths[b] on stay as they are; the call then takes
+ * 4 * batch * heads * max_length bytes of scratch.  head_dim up to 256.  An infinite
  * value (not key) in a slot that counts gives NaN or an infinity. */
 int mb_paged_attention(mb_context *ctx, const void *q, const void *k_cache,
                        const void *v_cache, const int32_t *page_table,
@@ -614,8 +615,8 @@ int mb_dequantize_mxfp4(mb_context *ctx, const uint8_t *codes,
 
 /* C[m][n] = sum_k A[m][k] B[n][k] (+ bias[n]), A [M][K] and B [N][K] both in
  * MXFP4 as above, bias fp32 (may be NULL), C in rows of `stride` elements of
- * the given type.  Products are exact, sums fp32.  codes and scales 16-byte
- * aligned. */
+ * the given type, apart from the operands.  Products are exact, sums fp32.
+ * codes and scales 16-byte aligned.  K = 0 gives the bias, or zeros. */
 int mb_gemm_mxfp4(mb_context *ctx, const uint8_t *a_codes,
                   const uint8_t *a_scales, const uint8_t *b_codes,
                   const uint8_t *b_scales, const float *bias, void *C,

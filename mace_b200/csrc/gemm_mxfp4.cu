@@ -158,18 +158,21 @@ gemm_mxfp4_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     tmem_alloc(smem_u32(tmem_slot), C::TMEM);
     tmem_relinquish();
   }
-  tc_fence_before_sync();
-  __syncthreads();
-  tc_fence_after_sync();
-  const uint32_t tmem = *tmem_slot;
-  mb_grid_dep_wait();
-
   // this CTA's tiles, and its run of their depth
   const int rank = p.splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int first = blockIdx.x / p.splits, stride = gridDim.x / p.splits;
   const int steps_all = (p.blocks + 7) / 8;
   const int step0 = static_cast<int>(static_cast<int64_t>(steps_all) * rank / p.splits);
   const int steps = static_cast<int>(static_cast<int64_t>(steps_all) * (rank + 1) / p.splits) - step0;
+  // The first tile's rows of B are asked for into L2 while the kernel in front, as a rule the tokens' quantization, still runs.  (Into L2
+  // only: should that kernel write them after all, L2 is where its writes go.  One token through 24 layers of 4096 x 4096: 10.06 -> 9.69 us a layer.)
+  if (warp == TMA_WARP && lane == 0)
+    for (int i = 0; i < min(steps, STAGES); ++i) tma_prefetch_3d(&map_b, (step0 + i) * 128, first % p.tiles_n * 128, 0);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  mb_grid_dep_wait();
   const auto fail = [&](int code) {
     *abort_flag = 1;
     atomicCAS(p.status, 0, code);

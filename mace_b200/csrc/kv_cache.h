@@ -89,6 +89,12 @@ inline Verdict check_pool(int64_t num_pages, int64_t page_size, int64_t kv_heads
   return fine();
 }
 
+// Whether two stretches of 4-byte values have none in common.
+inline bool apart(const void *a, int64_t na, const void *b, int64_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y ? (y - x) / 4 >= static_cast<uintptr_t>(na) : (x - y) / 4 >= static_cast<uintptr_t>(nb);
+}
+
 #define KV_PASS(expr)                              \
   do {                                             \
     const Verdict kv_v = (expr);                   \
@@ -192,7 +198,7 @@ inline Verdict check_evict(const void *k_src, const void *v_src, const int32_t *
   KV_REQUIRE(aligned(k_src, size) && aligned(v_src, size) && aligned(k_dst, size) && aligned(v_dst, size) && aligned(src_table, 4) &&
              aligned(dst_table, 4) && aligned(lengths, 4) && aligned(dst_lengths, 4) && aligned(weights, 4) &&
              aligned(dst_weights, 4) && aligned(kept, 4), "misaligned operand");
-  KV_REQUIRE(weights != dst_weights, "dst_weights may not be weights");
+  KV_REQUIRE(apart(weights, batch * kv_heads * weights_stride, dst_weights, batch * kv_heads * budget), "dst_weights may not lie in weights");
   return fine();
 }
 

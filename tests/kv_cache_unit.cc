@@ -37,7 +37,7 @@ struct Attention {
 struct Evict {
   const void *k = X, *v = X, *k_dst = Y, *v_dst = Y;
   const int32_t *table = I, *lengths = I, *dst_table = I, *dst_lengths = I, *kept = I;
-  const float *weights = F, *dst_weights = F + 1;
+  const float *weights = F, *dst_weights = F + 256;   // (2 x 2 x 64 weights)
   int64_t batch = 2, heads = 2, dim = 64, page = 16, pages = 10, max_pages = 4, dst_pages = 10, dst_max_pages = 2, max_length = 64,
           stride = 64, budget = 32, sinks = 4, recent = 8;
   int dtype = MB_F16;
@@ -132,6 +132,9 @@ int main() {
   EXPECT(with<Evict>([](Evict &e) { e.budget = 33; e.max_length = 32; }) == MB_SUCCESS);        // nothing longer to keep
   EXPECT(with<Evict>([](Evict &e) { e.stride = 63; }) == MB_INVALID_ARGS);
   EXPECT(with<Evict>([](Evict &e) { e.dst_weights = F; }) == MB_INVALID_ARGS);
+  EXPECT(with<Evict>([](Evict &e) { e.dst_weights = F + 255; }) == MB_INVALID_ARGS);
+  EXPECT(with<Evict>([](Evict &e) { e.dst_weights = F - 127; }) == MB_INVALID_ARGS);              // (2 x 2 x 32 kept)
+  EXPECT(with<Evict>([](Evict &e) { e.dst_weights = F - 128; }) == MB_SUCCESS);
   EXPECT(with<Evict>([](Evict &e) { e.kept = nullptr; }) == MB_INVALID_ARGS);
   EXPECT(with<Evict>([](Evict &e) { e.dst_table = nullptr; }) == MB_INVALID_ARGS);
   EXPECT(with<Evict>([](Evict &e) { e.k_dst = memory + 1; }) == MB_INVALID_ARGS);
