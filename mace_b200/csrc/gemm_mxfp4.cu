@@ -24,6 +24,7 @@ struct MxGemmParams {
   int64_t stride;
   int M, N, blocks, tiles;   // blocks of 32 and tiles of scales of a row
   int tiles_n, count, splits;
+  int words;         // C's rows are whole words of this many neighbouring values, aligned: 1, 2 or 4
   int *status;
 };
 
@@ -291,13 +292,30 @@ gemm_mxfp4_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         float *part = reinterpret_cast<float *>(smem) + half * C::HALF * 128 + quarter * 32 + lane;
 #pragma unroll
         for (int c = 0; c < C::HALF; ++c) part[c * 128] = __uint_as_float(r[c]) + bias;
-      } else if (n < p.N) {
+      } else {
         const int m0 = tm * BT + half * C::HALF, rows = p.M - m0;
-        T *to = static_cast<T *>(p.c) + m0 * p.stride + n;
+        if (sizeof(T) == 2 && p.words > 1) {
+          // two columns at a time: an even lane has the first one's values of itself and its neighbour, the odd one the second's
+          // (64 bytes of two rows each a store instead of one's)
+          const int odd = lane & 1;
+          T *to = static_cast<T *>(p.c) + (m0 + odd) * p.stride + (n - odd);
 #pragma unroll
-        for (int c = 0; c < C::HALF; ++c) {
-          if (c < rows) *to = elem::narrow<T>(__uint_as_float(r[c]) + bias);
-          to += p.stride;
+          for (int c = 0; c < C::HALF; c += 2) {
+            elem::Vec<T, 4 / sizeof(T)> mine;
+            mine.v[0] = elem::narrow<T>(__uint_as_float(r[c]) + bias);
+            mine.v[1 % (4 / sizeof(T))] = elem::narrow<T>(__uint_as_float(r[c + 1]) + bias);
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, mine.word, 1);
+            const uint32_t word = odd ? __byte_perm(other, mine.word, 0x7632) : __byte_perm(mine.word, other, 0x5410);
+            if (c + odd < rows && n < p.N) *reinterpret_cast<uint32_t *>(to) = word;
+            to += 2 * p.stride;
+          }
+        } else if (n < p.N) {
+          T *to = static_cast<T *>(p.c) + m0 * p.stride + n;
+#pragma unroll
+          for (int c = 0; c < C::HALF; ++c) {
+            if (c < rows) *to = elem::narrow<T>(__uint_as_float(r[c]) + bias);
+            to += p.stride;
+          }
         }
       }
     }
@@ -327,9 +345,16 @@ gemm_mxfp4_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         for (int j = 0; j < 4; ++j) sum[j] += v[j];
       }
       T *to = static_cast<T *>(p.c) + m * p.stride + n;
+      elem::Vec<T, 4> out;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (n + j < p.N) to[j] = elem::narrow<T>(sum[j]);
+      for (int j = 0; j < 4; ++j) out.v[j] = elem::narrow<T>(sum[j]);
+      if (p.words == 4) {
+        if (n < p.N) out.store(to);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < p.N) to[j] = out.v[j];
+      }
     }
     // no CTA of a cluster may leave while another still reads its tile
     cluster_sync_all();
@@ -410,6 +435,8 @@ extern "C" int mb_gemm_mxfp4(mb_context *ctx, const uint8_t *a_codes, const uint
   p.blocks = static_cast<int>(mx::blocks_of(K)); p.tiles = static_cast<int>(mx::tile_cols(K));
   p.tiles_n = static_cast<int>(ceil_div64(N, 128));
   p.status = ctx->dev_status;
+  const uintptr_t each = kv::type_bytes(dtype);
+  p.words = N % 4 == 0 && stride % 4 == 0 && kv::aligned(C, 4 * each) ? 4 : N % 2 == 0 && stride % 2 == 0 && kv::aligned(C, 2 * each) ? 2 : 1;
   if (ctx->use_tensor_cores && ctx->encode_tiled != nullptr && K > 0) {
     int st = MB_SUCCESS;
     MB_FOR_ELEMENT(dtype, st = gemm_tc<T>(ctx, p, dtype));

@@ -193,6 +193,19 @@ def test_gemm_every_code_and_scale_has_its_place(ctx, M, N, K):
         assert np.array_equal(got, want)
 
 
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("M,N,K", [(20, 132, 512), (300, 516, 96), (300, 518, 96), (3, 130, 1024)])
+@pytest.mark.parametrize("pad,offset", [(0, 0), (0, 1), (0, 2), (1, 0), (2, 0), (4, 4)])
+def test_gemm_rows_of_every_alignment(ctx, name, M, N, K, pad, offset):
+    """Stores of one, two and four values: the same bits, and nothing between the rows."""
+    rng = np.random.default_rng(N)
+    a, b = _random_mx(rng, M, K, 116, 128), _random_mx(rng, N, K, 116, 128)
+    bias = rng.standard_normal(N).astype(np.float32)
+    got = _gemm(ctx, a, b, bias, name, stride=N + pad, offset=offset)
+    _check(got, a, b, bias, name)
+    assert torch.equal(got, _gemm(ctx, a, b, bias, name))
+
+
 def test_gemm_nan_scale_and_empty_sum(ctx):
     rng = np.random.default_rng(5)
     a, b = _random_mx(rng, 20, 200), _random_mx(rng, 140, 200)
