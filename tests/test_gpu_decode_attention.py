@@ -142,6 +142,15 @@ def test_on_cuda_cores(ctx, name):
         ctx.set_option("tensor_cores", 1)
 
 
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,window", [
+    (4, 4, 128, 16, 0), (16, 4, 128, 32, 0), (64, 4, 128, 20, 0), (28, 4, 128, 16, 2000), (8, 8, 64, 16, 0), (40, 8, 64, 100, 4001), (160, 8, 64, 64, 0),
+    (12, 4, 256, 16, 0), (64, 4, 256, 16, 5000), (6, 6, 120, 16, 0), (7, 7, 99, 16, 0)])
+def test_runs_joined_through_memory(ctx, name, heads, kv_heads, dim, page, window):
+    """More than fits clusters: runs cut by the lengths, joined by the block that arrives last; empty and short sequences among long ones."""
+    Case(ctx, name, [9000, 0, 1, 4000, 8999, 130, 64], heads, kv_heads, dim, page, seed=dim + heads, window=window).run().check()
+
+
 @pytest.mark.parametrize("name", ["f32", "bf16"])
 @pytest.mark.parametrize("window", [1, 7, 64, 500, 100000])
 def test_window(ctx, name, window):

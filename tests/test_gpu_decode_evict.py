@@ -118,6 +118,18 @@ def test_long(ctx, kind, length, budget):
     check()
 
 
+@pytest.mark.parametrize("kind", ["spread", "ties", "special"])
+@pytest.mark.parametrize("batch,longest", [(80, 500), (160, 25000)])
+def test_more_heads_than_sms(ctx, kind, batch, longest):
+    rng = np.random.default_rng(batch)
+    lengths = [int(n) for n in rng.integers(0, 300, batch)]
+    lengths[3] = longest
+    heads = 2 if batch < 148 else 1
+    call, check = _case(ctx, "bf16", lengths, heads, 8, 16, 120, 4, 30, kind, seed=batch)
+    call()
+    check()
+
+
 def test_lengths_in_place_one_pool_and_twice(ctx):
     call, check = _case(ctx, "f32", [100, 20, 60], 2, 32, 8, 30, 2, 5, same_lengths=True, same_pool=True)
     call()
