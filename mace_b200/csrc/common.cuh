@@ -58,7 +58,7 @@ struct mb_context {
   void *op_scratch = nullptr, *op_counters = nullptr;
   size_t op_scratch_bytes = 0, op_counters_bytes = 0;
   std::vector<void *> op_kept;
-  uint32_t attention_attr_mask = 0;  // kernels of paged_attention.cu whose shared-memory limit was raised
+  uint64_t attention_attr_mask = 0;  // kernels of paged_attention.cu whose shared-memory limit was raised
   bool evict_attr_set = false;       // the same for kv_evict.cu
   uint32_t mxfp4_attr_mask = 0;      // the same for gemm_mxfp4.cu
   uint32_t f32_pairs_attr_mask = 0;  // kernels of gemm_f32_pairs.cu whose shared-memory limit was raised

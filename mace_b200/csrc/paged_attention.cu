@@ -598,8 +598,9 @@ struct Ring {
   static constexpr int STAGES = ROW == 256 ? 2 : 3;               // (two of 256-byte rows: three blocks an SM)
   static constexpr int BYTES = WARPS * STAGES * STAGE;
   static constexpr int PITCH = DIM + 4;                       // floats between rows of the accumulators at the end
-  static_assert(2 * 16 * MAX_SPLITS * 4 <= BYTES, "what joins the runs reuses it too");
-  static_assert(WARPS * 16 * PITCH * 4 <= BYTES, "accumulators reuse the ring");
+  static constexpr int MOST_HEADS = DIM * sizeof(T) <= 256 ? 24 : 16;
+  static_assert(2 * MOST_HEADS * MAX_SPLITS * 4 <= BYTES, "what joins the runs reuses it too");
+  static_assert(WARPS * MOST_HEADS * PITCH * 4 <= BYTES, "accumulators reuse the ring");
 };
 
 // Where the words of a row of values lie: 16-bit rows are read by ldmatrix, eight at a time; fp32 ones as single values, four rows of two
@@ -925,10 +926,10 @@ template <typename T, int DIM, int HEADS, bool WHOLE>
 int launch_mma(mb_context *ctx, const AttentionParams &p, unsigned grid, int index) {
   const auto kern = paged_attention_mma_kernel<T, DIM, HEADS, WHOLE>;
   index += (HEADS - 1) * 2 + WHOLE;
-  if (!(ctx->attention_attr_mask & (1u << index))) {
+  if (!(ctx->attention_attr_mask & (1ull << index))) {
     MB_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<T, DIM>::BYTES));
     MB_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));   // clusters of 16
-    ctx->attention_attr_mask |= 1u << index;
+    ctx->attention_attr_mask |= 1ull << index;
   }
   MB_CUDA(ctx, mb_launch_clusters(ctx, kern, grid, THREADS, Ring<T, DIM>::BYTES, p.cluster, p));
   return MB_SUCCESS;
@@ -937,6 +938,9 @@ int launch_mma(mb_context *ctx, const AttentionParams &p, unsigned grid, int ind
 template <typename T, int DIM>
 int launch_mma(mb_context *ctx, const AttentionParams &p, unsigned grid, int rows, int index) {
   const bool whole = p.dim == DIM && p.page_size % Ring<T, DIM>::CHUNK == 0;
+  if constexpr (sizeof(T) == 2 && DIM <= 128) {
+    if (rows > 16) return whole ? launch_mma<T, DIM, 3, true>(ctx, p, grid, index) : launch_mma<T, DIM, 3, false>(ctx, p, grid, index);
+  }
   if constexpr (sizeof(T) == 2) {
     if (rows > 8) return whole ? launch_mma<T, DIM, 2, true>(ctx, p, grid, index) : launch_mma<T, DIM, 2, false>(ctx, p, grid, index);
   }
@@ -946,8 +950,8 @@ int launch_mma(mb_context *ctx, const AttentionParams &p, unsigned grid, int row
 template <typename T>
 int launch_mma(mb_context *ctx, const AttentionParams &p, unsigned grid, int rows, int index) {
   if (p.dim <= 64) return launch_mma<T, 64>(ctx, p, grid, rows, index);
-  if (sizeof(T) == 4 || p.dim <= 128) return launch_mma<T, 128>(ctx, p, grid, rows, index + 4);
-  if constexpr (sizeof(T) == 2) return launch_mma<T, 256>(ctx, p, grid, rows, index + 8);
+  if (sizeof(T) == 4 || p.dim <= 128) return launch_mma<T, 128>(ctx, p, grid, rows, index + 6);
+  if constexpr (sizeof(T) == 2) return launch_mma<T, 256>(ctx, p, grid, rows, index + 12);
   return MB_SUCCESS;
 }
 
@@ -1030,7 +1034,10 @@ extern "C" int mb_paged_attention(mb_context *ctx, const void *q, const void *k_
   const bool f32 = dtype == MB_F32;
   const bool by_mma = ctx->use_tensor_cores && head_dim % (f32 ? 4 : 8) == 0 && (!f32 || head_dim <= 128) && kv::aligned(k_cache, 16) &&
                       kv::aligned(v_cache, 16);
-  const int rows = by_mma ? (p.group > 8 && !f32 ? 16 : 8) : p.group >= 5 ? 8 : p.group >= 3 ? 4 : p.group;
+  // Rows of a block: as many of a group's heads as registers hold, since every block of heads reads the run again (20 heads of 128 in one
+  // block of 24 142 us, in two of 16 171).
+  const bool three = by_mma && !f32 && head_dim <= 128 && (p.group + 23) / 24 < (p.group + 15) / 16;
+  const int rows = three ? 24 : by_mma ? (p.group > 8 && !f32 ? 16 : 8) : p.group >= 5 ? 8 : p.group >= 3 ? 4 : p.group;
   p.blocks = (p.group + rows - 1) / rows;
   p.batch = static_cast<int>(batch);
   p.pitch = static_cast<int>(align_up(p.dim, 4));
@@ -1044,7 +1051,7 @@ extern "C" int mb_paged_attention(mb_context *ctx, const void *q, const void *k_
   p.cluster = 1;
   if (units * p.longest * 2 * head_dim * kv::type_bytes(dtype) <= SMALL)
     while (p.cluster < most && units * p.cluster * 2 <= 2 * ctx->num_sms && p.longest > LEAST_RUN * p.cluster) p.cluster *= 2;
-  const int per_sm = !by_mma ? (rows * p.dim >= 1024 ? 3 : 5) : p.dim * kv::type_bytes(dtype) > 256 ? 1 : p.dim * kv::type_bytes(dtype) > 128 ? 3 : 4;
+  const int per_sm = three ? 2 : !by_mma ? (rows * p.dim >= 1024 ? 3 : 5) : p.dim * kv::type_bytes(dtype) > 256 ? 1 : p.dim * kv::type_bytes(dtype) > 128 ? 3 : 4;
   const int64_t slots = per_sm * ctx->num_sms;
   // one round of blocks where the heads leave it room, else several, so that the last one is a small part
   p.resident = static_cast<int>(std::min<int64_t>(units * 2 <= slots ? slots - units : 4 * slots, MAX_SPLITS * kv_heads * p.blocks));
@@ -1082,9 +1089,9 @@ extern "C" int mb_paged_attention(mb_context *ctx, const void *q, const void *k_
   const unsigned grid = static_cast<unsigned>(runs);
   cudaError_t e = cudaSuccess;
   if (by_mma) {
-    if (f32) MB_RETURN_IF_ERROR(launch_mma<float>(ctx, p, grid, rows, 24));
+    if (f32) MB_RETURN_IF_ERROR(launch_mma<float>(ctx, p, grid, rows, 36));
     else if (dtype == MB_F16) MB_RETURN_IF_ERROR(launch_mma<__half>(ctx, p, grid, rows, 0));
-    else MB_RETURN_IF_ERROR(launch_mma<__nv_bfloat16>(ctx, p, grid, rows, 12));
+    else MB_RETURN_IF_ERROR(launch_mma<__nv_bfloat16>(ctx, p, grid, rows, 18));
   } else MB_FOR_ELEMENT(dtype, {
     const uintptr_t word = 4 * sizeof(T);
     const bool vec = p.dim % 4 == 0 && q_stride % 4 == 0 && kv::aligned(q, word) && kv::aligned(k_cache, word) && kv::aligned(v_cache, word);

@@ -81,7 +81,7 @@ class Case:
                     assert (weights[b, h, n:] == -5.0).all()
 
 
-HEADS = [(1, 1), (2, 1), (3, 1), (8, 2), (8, 8), (14, 2), (32, 4), (20, 1), (40, 1)]
+HEADS = [(1, 1), (2, 1), (3, 1), (8, 2), (8, 8), (14, 2), (32, 4), (17, 1), (20, 1), (24, 1), (32, 1), (40, 1), (56, 1)]
 
 
 @pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
