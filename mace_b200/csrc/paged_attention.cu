@@ -36,7 +36,7 @@ struct AttentionParams {
   const float *weights_in;
   float *weights_out;
   int64_t q_stride, out_stride, num_pages, logits_stride, weights_stride, window;
-  int batch, heads, kv_heads, group, blocks, dim, pitch, page_size, max_pages, longest, resident;
+  int batch, heads, kv_heads, group, blocks, dim, pitch, page_size, max_pages, longest, wanted;   // wanted: runs, about
   int cluster;                 // above 1: every head's slots over a cluster of so many blocks
   int fixed_runs, fixed_run;   // batches above SCANNED: every head has so many runs of so many slots
   uint32_t page_mul, page_shift;
@@ -48,7 +48,7 @@ struct AttentionParams {
 // heads over the blocks that are resident at once give a run's length, a sequence has as many runs as it needs, and a
 // prefix sum over the sequences says whose run this block's is.  No block is without work but the few behind the last run, and a
 // batch of one long and many short sequences fills the SMs as well as one of equals.  (Runs cut by the longest sequence, which
-// the host knows: a batch of 32 from 1 to 4096 slots took 57 us instead of 51.)
+// the host knows: a batch of 32 from 1 to 4096 slots took 57 us instead of 49.)
 struct Place {
   int unit, batch, kv_head, head0, heads, split, active, first, begin, end;   // slots from `first` on; the run is begin .. end
   int record;                                                                 // of the unit's first run; the next ones p.blocks apart
@@ -72,7 +72,7 @@ struct Place {
   // false: there is no such run.
   __device__ __forceinline__ bool find(const AttentionParams &p, int rows, int chunk) {
     __shared__ long long sums[WARPS];
-    __shared__ int counts[WARPS], found[2];
+    __shared__ int tops[WARPS], counts[WARPS], found[2];
     const int t = threadIdx.x, lane = t % 32, warp = t / 32, per_run = p.kv_heads * p.blocks;
     int from;
     bool bad;
@@ -111,17 +111,28 @@ struct Place {
       return true;
     }
     long long total = 0;
+    int top = 0;
     for (int b = t; b < p.batch; b += THREADS) {
-      total += slots_of(p, b, chunk, &first, &from, &bad);
+      const int slots = slots_of(p, b, chunk, &first, &from, &bad);
+      total += slots;
+      top = max(top, slots);
       if (bad && blockIdx.x == 0) mb_report_bad_index(p.status);
     }
+    top = static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<unsigned>(top)));
 #pragma unroll
     for (int o = 16; o > 0; o /= 2) total += __shfl_xor_sync(0xffffffffu, total, o);
-    if (lane == 0) sums[warp] = total;
+    if (lane == 0) {
+      sums[warp] = total;
+      tops[warp] = top;
+    }
     __syncthreads();
     total = 0;
-    for (int w = 0; w < WARPS; ++w) total += sums[w];
-    const long long share = (total * per_run + p.resident - 1) / p.resident;
+    for (int w = 0; w < WARPS; ++w) {
+      total += sums[w];
+      top = max(top, tops[w]);
+    }
+    // (no sequence may have more than MAX_SPLITS runs)
+    const long long share = max((total * per_run + p.wanted - 1) / p.wanted, static_cast<long long>((top + MAX_SPLITS - 1) / MAX_SPLITS));
     const int most = static_cast<int>(min(max(static_cast<long long>(LEAST_RUN), (share + 63) / 64 * 64), 0x7fffffc0ll));
     int before = 0;   // runs of the sequences in front of this round's
     for (int base = 0; base < p.batch; base += THREADS) {
@@ -1041,8 +1052,6 @@ extern "C" int mb_paged_attention(mb_context *ctx, const void *q, const void *k_
   p.blocks = (p.group + rows - 1) / rows;
   p.batch = static_cast<int>(batch);
   p.pitch = static_cast<int>(align_up(p.dim, 4));
-  // As many runs as blocks are resident, and one more for each head of a sequence, whose last run is not a whole one; a sequence of one
-  // run is all that short ones have.
   const int64_t units = batch * kv_heads * p.blocks;
   // Work that is over before its blocks' parts could meet in memory: each head's slots over a cluster, 128 of them a block at least
   // (1000 slots, 8 heads: 10.4 us with the runs joined by the last block, 7.7 on clusters of 8; 8192: 18.6 and 16.1 on 16).
@@ -1052,10 +1061,12 @@ extern "C" int mb_paged_attention(mb_context *ctx, const void *q, const void *k_
   if (units * p.longest * 2 * head_dim * kv::type_bytes(dtype) <= SMALL)
     while (p.cluster < most && units * p.cluster * 2 <= 2 * ctx->num_sms && p.longest > LEAST_RUN * p.cluster) p.cluster *= 2;
   const int per_sm = three ? 2 : !by_mma ? (rows * p.dim >= 1024 ? 3 : 5) : p.dim * kv::type_bytes(dtype) > 256 ? 1 : p.dim * kv::type_bytes(dtype) > 128 ? 3 : 4;
-  const int64_t slots = per_sm * ctx->num_sms;
-  // one round of blocks where the heads leave it room, else several, so that the last one is a small part
-  p.resident = static_cast<int>(std::min<int64_t>(units * 2 <= slots ? slots - units : 4 * slots, MAX_SPLITS * kv_heads * p.blocks));
-  int64_t runs = std::min<int64_t>(units + p.resident, units * std::max<int64_t>(1, ceil_div64(p.longest + 15, LEAST_RUN)));
+  // The runs wanted of all heads together: one round of resident blocks where the heads leave room for it, less one for each head, whose
+  // last run is not a whole one; else half as many again as are resident.  (256 heads of 4096 slots, 444 blocks resident: 444 wanted
+  // 105 us, 666 90, 888 97; 512 ragged ones of up to 8192: 168, 164, 164.  As many as fill the last round, up to 8 of them: 94 and 173.)
+  const int64_t slots = static_cast<int64_t>(per_sm) * ctx->num_sms;
+  p.wanted = static_cast<int>(units * 2 <= slots ? slots - units : slots * 3 / 2);
+  int64_t runs = std::min<int64_t>(units + p.wanted, units * std::max<int64_t>(1, ceil_div64(p.longest + 15, LEAST_RUN)));
   if (p.cluster > 1) {
     runs = units * p.cluster;
   } else if (batch > SCANNED) {
