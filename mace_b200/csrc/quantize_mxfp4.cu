@@ -12,7 +12,8 @@ namespace {
 
 constexpr int THREADS = 256;
 constexpr int EACH = 8;    // values of a thread at a time
-constexpr int TIMES = 4;   // groups of them, THREADS apart, so that addresses are worked out once and four loads are in flight
+// Groups of them that a thread has, THREADS apart (TIMES, a template's argument): addresses are worked out once, and as many loads are
+// in flight.  Four, or two where a row's end would leave half of a block without work.
 
 struct MxParams {
   const void *x;
@@ -22,6 +23,7 @@ struct MxParams {
   int cols, tiles;       // tiles of scales in a row of tiles
   int chunks;            // groups of EACH values in a row's tiles
   int vec;               // words of 16 bytes (fp32: two of them) are aligned
+  int times;
   int block_rows, row_blocks;   // a block has block_rows rows at a time, or (row_blocks > 0) a row so many blocks
   uint32_t chunk_mul, chunk_shift, row_mul, row_shift;
 };
@@ -99,7 +101,7 @@ __device__ __forceinline__ float2 values_of(uint32_t byte) {
 
 // Where a thread's groups lie.  WIDE: a row has one or more blocks, and the thread groups chunk, chunk + THREADS, .. of it; else a block
 // has several rows, and the thread the same group of rows block_rows apart.
-template <bool WIDE>
+template <bool WIDE, int TIMES>
 struct Span {
   int64_t row;
   int chunk;
@@ -133,11 +135,11 @@ struct Span {
 
 // Items are (row, group of eight) of the whole tiles: a lane whose block does not exist writes the tile's zeros.  Rows are whole groups
 // of sixteen lanes, whose four scales leave as a word.
-template <typename T, bool WIDE>
+template <typename T, bool WIDE, int TIMES>
 __global__ void __launch_bounds__(THREADS) quantize_mxfp4_kernel(const MxParams p) {
   mb_grid_dep_launch();
   mb_grid_dep_wait();
-  const Span<WIDE> at(p);
+  const Span<WIDE, TIMES> at(p);
   const int blocks = static_cast<int>(mx::blocks_of(p.cols));
   const int64_t tile_rows = mx::tile_rows(p.rows) * mx::TILE_ROWS;
   const T *x0 = static_cast<const T *>(p.x) + at.row * p.stride + at.chunk * EACH;
@@ -178,11 +180,11 @@ __global__ void __launch_bounds__(THREADS) quantize_mxfp4_kernel(const MxParams 
   }
 }
 
-template <typename T, bool WIDE>
+template <typename T, bool WIDE, int TIMES>
 __global__ void __launch_bounds__(THREADS) dequantize_mxfp4_kernel(const MxParams p) {
   mb_grid_dep_launch();
   mb_grid_dep_wait();
-  const Span<WIDE> at(p);
+  const Span<WIDE, TIMES> at(p);
   const int blocks = static_cast<int>(mx::blocks_of(p.cols));
   T *y0 = static_cast<T *>(p.y) + at.row * p.stride + at.chunk * EACH;
   uint32_t *codes0 = reinterpret_cast<uint32_t *>(p.codes) + at.row * blocks * 4 + at.chunk;
@@ -232,9 +234,11 @@ MxParams make(const void *x, void *y, uint8_t *codes, uint8_t *scales, int64_t r
   p.cols = static_cast<int>(cols);
   p.tiles = static_cast<int>(mx::tile_cols(cols));
   p.chunks = p.tiles * (mx::TILE_BLOCKS * mx::BLOCK / EACH);
-  // a row of THREADS groups or more has blocks of its own; shorter ones share one
+  // a row of more than THREADS groups has blocks of its own; shorter ones share one
   p.block_rows = std::max(1, THREADS / p.chunks);
-  p.row_blocks = p.chunks < THREADS ? 0 : (p.chunks + THREADS * TIMES - 1) / (THREADS * TIMES);
+  const int fours = (p.chunks + 4 * THREADS - 1) / (4 * THREADS), twos = (p.chunks + 2 * THREADS - 1) / (2 * THREADS);
+  p.times = p.chunks > THREADS && twos < 2 * fours ? 2 : 4;   // (4096 columns: 18.4 us with four for 4099 rows, 13.5 with two)
+  p.row_blocks = p.chunks <= THREADS ? 0 : p.times == 2 ? twos : fours;
   fast_div_make(p.chunks, &p.chunk_mul, &p.chunk_shift);
   fast_div_make(p.row_blocks, &p.row_mul, &p.row_shift);
   const void *values = x != nullptr ? x : y;
@@ -243,7 +247,7 @@ MxParams make(const void *x, void *y, uint8_t *codes, uint8_t *scales, int64_t r
 }
 
 int64_t blocks_for(const MxParams &p, int64_t rows) {
-  return p.row_blocks == 0 ? ceil_div64(rows, static_cast<int64_t>(p.block_rows) * TIMES) : rows * p.row_blocks;
+  return p.row_blocks == 0 ? ceil_div64(rows, static_cast<int64_t>(p.block_rows) * p.times) : rows * p.row_blocks;
 }
 
 }  // namespace
@@ -264,7 +268,7 @@ int mb_quantize_mxfp4(mb_context *ctx, const void *x, uint8_t *codes, uint8_t *s
   const MxParams p = make(x, nullptr, codes, scales, rows, cols, stride, dtype);
   const int64_t blocks = blocks_for(p, mx::tile_rows(rows) * mx::TILE_ROWS);
   if (blocks > kv::MOST) return mb_fail(ctx, MB_UNSUPPORTED, "mb_quantize_mxfp4: tensor too large");
-  MB_FOR_ELEMENT(dtype, MB_CUDA(ctx, mb_launch_chained(ctx, p.row_blocks > 0 ? quantize_mxfp4_kernel<T, true> : quantize_mxfp4_kernel<T, false>,
+  MB_FOR_ELEMENT(dtype, MB_CUDA(ctx, mb_launch_chained(ctx, p.row_blocks == 0 ? quantize_mxfp4_kernel<T, false, 4> : p.times == 2 ? quantize_mxfp4_kernel<T, true, 2> : quantize_mxfp4_kernel<T, true, 4>,
                                                        dim3(static_cast<unsigned>(blocks)), dim3(THREADS), 0, p)));
   ctx->launches++;
   return MB_SUCCESS;
@@ -280,7 +284,7 @@ int mb_dequantize_mxfp4(mb_context *ctx, const uint8_t *codes, const uint8_t *sc
   const MxParams p = make(nullptr, x, const_cast<uint8_t *>(codes), const_cast<uint8_t *>(scales), rows, cols, stride, dtype);
   const int64_t blocks = blocks_for(p, rows);
   if (blocks > kv::MOST) return mb_fail(ctx, MB_UNSUPPORTED, "mb_dequantize_mxfp4: tensor too large");
-  MB_FOR_ELEMENT(dtype, MB_CUDA(ctx, mb_launch_chained(ctx, p.row_blocks > 0 ? dequantize_mxfp4_kernel<T, true> : dequantize_mxfp4_kernel<T, false>,
+  MB_FOR_ELEMENT(dtype, MB_CUDA(ctx, mb_launch_chained(ctx, p.row_blocks == 0 ? dequantize_mxfp4_kernel<T, false, 4> : p.times == 2 ? dequantize_mxfp4_kernel<T, true, 2> : dequantize_mxfp4_kernel<T, true, 4>,
                                                        dim3(static_cast<unsigned>(blocks)), dim3(THREADS), 0, p)));
   ctx->launches++;
   return MB_SUCCESS;

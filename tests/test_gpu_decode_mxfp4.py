@@ -36,7 +36,8 @@ def _quantize(ctx, x, name, stride=None, offset=0):
 @pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("rows,cols,stride,offset", [
     (1, 1, None, 0), (1, 32, None, 0), (3, 33, None, 0), (130, 100, None, 0), (128, 256, None, 0), (257, 640, 641, 0), (5, 1000, 1008, 1),
-    (2, 4096, None, 0), (129, 31, 40, 8)])
+    (2, 4096, None, 0), (129, 31, 40, 8), (6, 2048, None, 0), (7, 2049, 2056, 0), (3, 3999, None, 1), (3, 6000, 6008, 0), (2, 8192, None, 0),
+    (5, 9000, None, 0), (2, 20000, None, 0)])
 def test_quantize_and_back(ctx, name, rows, cols, stride, offset):
     rng = np.random.default_rng(rows + cols)
     x = tensor(rng, name, rows, cols) * torch.from_numpy(np.exp2(rng.integers(-9, 9, (rows, 1)))).to(TYPES[name][1])
