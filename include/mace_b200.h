@@ -524,8 +524,8 @@ int mb_rope(mb_context *ctx, const void *x, void *y, const int32_t *positions,
  * row slots[t] % page_size).  A negative slot leaves its token out of the
  * cache (padding of a batch); q is rotated all the same.  Token strides in
  * elements, heads contiguous (q, k and v may be parts of one row).  Slots that
- * are not negative must differ from one another; which of two tokens stays in
- * a slot named twice is not defined. */
+ * are not negative must differ from one another; what a slot named twice
+ * holds is not defined. */
 int mb_rope_kv_append(mb_context *ctx, const void *q, void *q_out,
                       const void *k, const void *v, void *k_cache,
                       void *v_cache, const int32_t *positions,
@@ -572,7 +572,8 @@ int mb_paged_attention(mb_context *ctx, const void *q, const void *k_cache,
  * counts as less than everything).  A shorter sequence keeps all.  What is kept stays
  * in order and is copied to slots 0, 1, ... of the destination: pages of
  * k_dst / v_dst named by dst_table (the pools may be the source pools, the
- * pages may not be pages that the call reads).  Device memory is written as
+ * pages may not be pages that the call reads, and no page may be named twice;
+ * source pages may be shared between sequences).  Device memory is written as
  * follows, all of it only up to the new length min(lengths[b], budget):
  *   dst_lengths [batch]                     the new lengths (may be lengths)
  *   dst_weights [batch][kv_heads][budget]   the weights of the kept slots
