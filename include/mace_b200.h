@@ -580,7 +580,12 @@ int mb_paged_attention(mb_context *ctx, const void *q, const void *k_cache,
  *   kept        [batch][kv_heads][budget]   their old slots, ascending; here
  *                                           entries from the new length on
  *                                           become -1
- * weights: [batch][kv_heads][weights_stride].  sinks + recent <= budget. */
+ * weights: [batch][kv_heads][weights_stride].  sinks + recent <= budget.
+ *
+ * mb_kv_evict_strided: the same with dst_weights [batch][kv_heads]
+ * [dst_weights_stride], dst_weights_stride >= budget, whose entries from the
+ * new length on become 0: what the next steps' mb_paged_attention takes as
+ * weights_in and weights_out while the sequence grows again. */
 int mb_kv_evict(mb_context *ctx, const void *k_src, const void *v_src,
                 const int32_t *src_table, const int32_t *lengths,
                 const float *weights, void *k_dst, void *v_dst,
@@ -591,6 +596,17 @@ int mb_kv_evict(mb_context *ctx, const void *k_src, const void *v_src,
                 int64_t dst_max_pages, int64_t max_length,
                 int64_t weights_stride, int64_t budget, int64_t sinks,
                 int64_t recent, int dtype);
+int mb_kv_evict_strided(mb_context *ctx, const void *k_src, const void *v_src,
+                        const int32_t *src_table, const int32_t *lengths,
+                        const float *weights, void *k_dst, void *v_dst,
+                        const int32_t *dst_table, int32_t *dst_lengths,
+                        float *dst_weights, int32_t *kept, int64_t batch,
+                        int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                        int64_t src_pages, int64_t src_max_pages,
+                        int64_t dst_pages, int64_t dst_max_pages,
+                        int64_t max_length, int64_t weights_stride,
+                        int64_t dst_weights_stride, int64_t budget,
+                        int64_t sinks, int64_t recent, int dtype);
 
 /* 4-bit microscaled floating point (OCP MX, MXFP4): a row is cut into blocks
  * of 32 values, each held as a shared power of two 2^(s - 127), s a byte

@@ -112,6 +112,7 @@ PROTOTYPES = {
     "mb_rope_kv_append": (_int, [_vp] * 10 + [_i64] * 11 + [_int, _f32, _int]),
     "mb_paged_attention": (_int, [_vp] * 10 + [_i64] * 12 + [_f32, _int]),
     "mb_kv_evict": (_int, [_vp] * 12 + [_i64] * 13 + [_int]),
+    "mb_kv_evict_strided": (_int, [_vp] * 12 + [_i64] * 14 + [_int]),
     "mb_mxfp4_scale_bytes": (_sz, [_i64] * 2),
     "mb_quantize_mxfp4": (_int, [_vp] * 4 + [_i64] * 3 + [_int]),
     "mb_dequantize_mxfp4": (_int, [_vp] * 4 + [_i64] * 3 + [_int]),
@@ -429,7 +430,14 @@ class Context:
 
     def kv_evict(self, k_src, v_src, src_table, lengths, weights, k_dst, v_dst, dst_table, dst_lengths, dst_weights, kept,
                  batch, kv_heads, head_dim, page_size, src_pages, src_max_pages, dst_pages, dst_max_pages, max_length,
-                 weights_stride, budget, sinks, recent, dtype):
+                 weights_stride, budget, sinks, recent, dtype, dst_weights_stride=None):
+        """dst_weights_stride: rows of dst_weights longer than budget, zero behind the new length."""
+        if dst_weights_stride is not None:
+            self._check(_ops.mb_kv_evict_strided(self._p, k_src.ptr, v_src.ptr, src_table.ptr, lengths.ptr, weights.ptr,
+                k_dst.ptr, v_dst.ptr, dst_table.ptr, dst_lengths.ptr, dst_weights.ptr, kept.ptr, batch, kv_heads, head_dim,
+                page_size, src_pages, src_max_pages, dst_pages, dst_max_pages, max_length, weights_stride,
+                dst_weights_stride, budget, sinks, recent, dtype))
+            return
         self._check(_ops.mb_kv_evict(self._p, k_src.ptr, v_src.ptr, src_table.ptr, lengths.ptr, weights.ptr, k_dst.ptr,
             v_dst.ptr, dst_table.ptr, dst_lengths.ptr, dst_weights.ptr, kept.ptr, batch, kv_heads, head_dim, page_size,
             src_pages, src_max_pages, dst_pages, dst_max_pages, max_length, weights_stride, budget, sinks, recent, dtype))

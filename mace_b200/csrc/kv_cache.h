@@ -176,7 +176,8 @@ inline Verdict check_evict(const void *k_src, const void *v_src, const int32_t *
                            const void *k_dst, const void *v_dst, const int32_t *dst_table, const int32_t *dst_lengths,
                            const float *dst_weights, const int32_t *kept, int64_t batch, int64_t kv_heads, int64_t dim,
                            int64_t page_size, int64_t src_pages, int64_t src_max_pages, int64_t dst_pages, int64_t dst_max_pages,
-                           int64_t max_length, int64_t weights_stride, int64_t budget, int64_t sinks, int64_t recent, int dtype) {
+                           int64_t max_length, int64_t weights_stride, int64_t budget, int64_t sinks, int64_t recent, int dtype,
+                           int64_t dst_weights_stride = 0 /* rows of budget */) {
   KV_PASS(check_heads(batch, kv_heads, dim, dtype));
   KV_PASS(check_pool(src_pages, page_size, kv_heads, dim));
   KV_PASS(check_pool(dst_pages, page_size, kv_heads, dim));
@@ -188,6 +189,8 @@ inline Verdict check_evict(const void *k_src, const void *v_src, const int32_t *
   const int64_t longest = longest_of(max_length, src_max_pages, page_size), stays = budget < longest ? budget : longest;
   KV_REQUIRE(dst_max_pages * page_size >= stays, "the destination's table has no room for budget slots");
   KV_REQUIRE(weights_stride >= longest && weights_stride <= MOST, "weights_stride below the longest sequence, or too large");
+  if (dst_weights_stride == 0) dst_weights_stride = budget;
+  KV_REQUIRE(dst_weights_stride >= budget && dst_weights_stride <= MOST, "dst_weights_stride below budget, or too large");
   if (batch * kv_heads > MOST / 16 || batch * kv_heads > (MOST << 12) / budget) return unsupported("too many kv heads");
   if (batch == 0) return fine();
   KV_REQUIRE(lengths != nullptr && dst_lengths != nullptr && kept != nullptr && dst_weights != nullptr && weights != nullptr &&
@@ -198,7 +201,7 @@ inline Verdict check_evict(const void *k_src, const void *v_src, const int32_t *
   KV_REQUIRE(aligned(k_src, size) && aligned(v_src, size) && aligned(k_dst, size) && aligned(v_dst, size) && aligned(src_table, 4) &&
              aligned(dst_table, 4) && aligned(lengths, 4) && aligned(dst_lengths, 4) && aligned(weights, 4) &&
              aligned(dst_weights, 4) && aligned(kept, 4), "misaligned operand");
-  KV_REQUIRE(apart(weights, batch * kv_heads * weights_stride, dst_weights, batch * kv_heads * budget), "dst_weights may not lie in weights");
+  KV_REQUIRE(apart(weights, batch * kv_heads * weights_stride, dst_weights, batch * kv_heads * dst_weights_stride), "dst_weights may not lie in weights");
   return fine();
 }
 

@@ -79,6 +79,7 @@ PyMethodDef kMethods[] = {
     MB_ENTRY(mb_rope_kv_append),
     MB_ENTRY(mb_paged_attention),
     MB_ENTRY(mb_kv_evict),
+    MB_ENTRY(mb_kv_evict_strided),
     MB_ENTRY(mb_quantize_mxfp4),
     MB_ENTRY(mb_dequantize_mxfp4),
     MB_ENTRY(mb_gemm_mxfp4),

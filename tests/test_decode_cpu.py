@@ -76,3 +76,8 @@ def test_rope_frequencies_refuse():
         with pytest.raises(capi.MaceB200Error) as e:
             capi.rope_frequencies(**{"rotary_dim": 64, **kw})
         assert e.value.code == 1, kw
+
+
+def test_eviction_with_strided_weights_wants_a_context():
+    import mace_b200
+    assert mace_b200.lib().mb_kv_evict_strided(*[None] * 12, *[1] * 14, 0) == 1

@@ -196,3 +196,130 @@ def test_refusals(ctx):
         assert e.value.code == 1, kw
     call(batch=0)
     ctx.sync()
+
+
+@pytest.mark.parametrize("name,heads,dim,budget,extra", [("bf16", 2, 64, 50, 41), ("f32", 3, 20, 64, 0), ("f16", 1, 128, 300, 7000)])
+@pytest.mark.parametrize("same_lengths", [False, True])
+def test_weights_as_the_next_step_takes_them(ctx, name, heads, dim, budget, extra, same_lengths):
+    """Rows of weights longer than the budget: the kept ones in front, zeros behind, nothing beyond the last row."""
+    rng = np.random.default_rng(budget)
+    lengths, page = [200, 0, 31, budget, budget + 1, 999], 16
+    batch, longest, row = len(lengths), max(lengths), budget + extra
+    k, v, table, rows = paged(rng, name, lengths, heads, dim, page)
+    w = rng.random((batch, heads, longest)).astype(np.float32)
+    width = -(-budget // page)
+    new_table = rng.permutation(batch * width).reshape(batch, width).astype(np.int32)
+    dk, dv = Values(ctx, k), Values(ctx, v)
+    dk2, dv2 = (Values(ctx, torch.full((batch * width, heads, page, dim), 5.0, dtype=k.dtype)) for _ in range(2))
+    dn = Values(ctx, torch.tensor(lengths, dtype=torch.int32))
+    dn2 = dn if same_lengths else Values(ctx, torch.zeros(batch, dtype=torch.int32))
+    dw, dt, dt2 = ctx.upload(w), ctx.upload(table), ctx.upload(new_table)
+    dw2, kept = Values(ctx, torch.full((batch * heads * row + 9,), -3.0)), Values(ctx, torch.zeros(batch, heads, budget, dtype=torch.int32))
+    ctx.kv_evict(dk, dv, dt, dn, dw, dk2, dv2, dt2, dn2, dw2, kept, batch, heads, dim, page, k.shape[0], table.shape[1], batch * width, width,
+                 longest, longest, budget, 4, 10, TYPES[name][0], dst_weights_stride=row)
+    ctx.sync()
+    got = dw2.get().numpy()
+    assert (got[batch * heads * row:] == -3.0).all() and dn2.get().tolist() == [min(n, budget) for n in lengths]
+    got = got[:batch * heads * row].reshape(batch, heads, row)
+    new_k = dk2.get()
+    for b, n in enumerate(lengths):
+        for h in range(heads):
+            want = choose(w[b, h, :n], budget, 4, 10)
+            m = len(want)
+            assert kept.get()[b, h, :m].tolist() == want and (kept.get()[b, h, m:] == -1).all()
+            assert np.array_equal(got[b, h, :m], w[b, h, want]) and (got[b, h, m:] == 0.0).all()
+            j = np.arange(m)
+            assert torch.equal(new_k[torch.from_numpy(new_table[b, j // page].astype(np.int64)), h, torch.from_numpy(j % page)], rows[b][0][want, h])
+
+
+def test_evicted_again_and_again_from_a_graph(ctx):
+    """Two evictions, to and fro between two sets of pages and of weights, captured once and replayed: attention's weights need no
+    rearranging in between."""
+    import ctypes as C
+
+    from mace_b200.capi import lib
+    L = lib()
+    rng = np.random.default_rng(3)
+    batch, heads, kv_heads, dim, page, room, budget, name = 3, 4, 2, 64, 16, 96, 40, "f32"
+    lengths = [90, 41, 17]
+    width = room // page
+    pages = 2 * batch * width
+    tables = rng.permutation(pages).reshape(2, batch, width).astype(np.int32)
+    k, v = (torch.from_numpy(rng.standard_normal((pages, kv_heads, page, dim)).astype(np.float32)) for _ in range(2))
+    w = np.zeros((batch, kv_heads, room), np.float32)
+    for b, n in enumerate(lengths):
+        w[b, :, :n] = rng.random((kv_heads, n))
+    q = torch.from_numpy(rng.standard_normal((batch, heads, dim)).astype(np.float32))
+    dk, dv, dq, out = Values(ctx, k), Values(ctx, v), Values(ctx, q), Values(ctx, q)
+    dn, dt = Values(ctx, torch.tensor(lengths, dtype=torch.int32)), [ctx.upload(t) for t in tables]
+    dw = [Values(ctx, torch.from_numpy(w)), Values(ctx, torch.full((batch, kv_heads, room), -1.0))]
+    kept = Values(ctx, torch.zeros(batch, kv_heads, budget, dtype=torch.int32))
+
+    def attend(i):
+        ctx.paged_attention(dq, dk, dv, dt[i], dn, out, batch, heads, kv_heads, dim, pages, page, width, room, 0.125, 0, weights_in=dw[i],
+                            weights_out=dw[i], weights_stride=room)
+
+    def evict(i, n):
+        ctx.kv_evict(dk, dv, dt[i], dn, dw[i], dk, dv, dt[1 - i], dn, dw[1 - i], kept, batch, kv_heads, dim, page, pages, width, pages, width,
+                     room, room, n, 2, 5, 0, dst_weights_stride=room)
+
+    def both():
+        attend(0)
+        evict(0, budget)
+        attend(1)
+        evict(1, budget - 8)
+
+    # the same by hand
+    def host(times):
+        rows = [[[(k[torch.from_numpy(tables[0][b][j // page:j // page + 1].astype(np.int64))[0], h, j % page],
+                   v[torch.from_numpy(tables[0][b][j // page:j // page + 1].astype(np.int64))[0], h, j % page], float(w[b, h, j]))
+                  for j in range(lengths[b])] for h in range(kv_heads)] for b in range(batch)]
+        for step in range(2 * times):
+            for b in range(batch):
+                for h in range(kv_heads):
+                    r = rows[b][h]
+                    keys = torch.stack([x[0] for x in r]).double()
+                    p = torch.softmax(q[b, 2 * h:2 * h + 2].double() @ keys.T * 0.125, 1).sum(0)
+                    r = [(x[0], x[1], x[2] + float(y)) for x, y in zip(r, p)]
+                    rows[b][h] = [r[j] for j in choose(np.array([x[2] for x in r]), budget - 8 * (step % 2), 2, 5)]
+        return rows
+
+    def check(times):
+        rows = host(times)
+        got_k, got_w, n = dk.get(), dw[0].get().numpy(), dn.get().tolist()
+        for b in range(batch):
+            for h in range(kv_heads):
+                r = rows[b][h]
+                assert n[b] == len(r)
+                for j, x in enumerate(r):
+                    assert torch.equal(got_k[int(tables[0][b][j // page]), h, j % page], x[0])
+                # fp32: (dim + 16) roundings of a logit of at most 8 or so, twice, for each of the steps
+                assert np.allclose(got_w[b, h, :len(r)], [x[2] for x in r], rtol=0, atol=2 * times * 2 * (dim + 16) * 8 * 2.0 ** -23)
+                assert (got_w[b, h, len(r):] == 0.0).all()
+
+    both()
+    ctx.sync()
+    check(1)
+    assert L.mb_graph_begin(ctx.h) == 0
+    both()
+    graph = C.c_void_p()
+    assert L.mb_graph_end(ctx.h, C.byref(graph)) == 0
+    for _ in range(3):
+        assert L.mb_graph_launch(ctx.h, graph) == 0
+    ctx.sync()
+    check(4)
+    L.mb_graph_destroy(ctx.h, graph)
+
+
+def test_refusals_of_strided_weights(ctx):
+    from mace_b200 import MaceB200Error
+    x, y = Values(ctx, torch.zeros(64)), Values(ctx, torch.zeros(64))
+    for stride in (0, -1, 3, 2 ** 31):
+        with pytest.raises(MaceB200Error) as e:
+            ctx.kv_evict(x, x, x, x, x, y, y, x, y, y, y, 1, 1, 8, 4, 2, 2, 2, 1, 8, 8, 4, 1, 1, 0, dst_weights_stride=stride)
+        assert e.value.code == 1 and "dst_weights_stride" in str(e.value)
+    with pytest.raises(MaceB200Error) as e:     # the rows' tail reaches into weights
+        class Before:
+            ptr = x.ptr - 16
+        ctx.kv_evict(x, x, x, x, x, y, y, x, y, Before, y, 1, 1, 8, 4, 2, 2, 2, 1, 8, 8, 4, 1, 1, 0, dst_weights_stride=8)
+    assert e.value.code == 1 and "dst_weights" in str(e.value)
