@@ -24,6 +24,12 @@ constexpr int LEAST_RUN = 128;   // slots that are worth a block of their own (1
 constexpr int SCANNED = 1024;    // sequences whose lengths every block reads
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
+// What a probability is multiplied by until the end, relative to one of the running maximum.  Halves reach from 2^-24 to 2^16 only, and
+// most probabilities are small: the largest are brought to their upper end.
+template <typename T> constexpr int LIFT = 0;   // as a power of two
+template <> constexpr int LIFT<__half> = 15;
+template <typename T> constexpr float RAISED = static_cast<float>(1 << LIFT<T>);
+
 struct AttentionParams {
   const void *q, *k, *v;
   const int32_t *table, *lengths;
@@ -205,10 +211,11 @@ __device__ __forceinline__ float load_remote(uint32_t addr, int rank) {
   return v;
 }
 
-// The log-sum-exp of the block's row h, for the caller and for the weights.
+// The log-sum-exp of the block's row h, for the caller and for the weights.  l: the sum as it was kept.
+template <typename T>
 __device__ __forceinline__ void tell(const AttentionParams &p, const Place &at, int h, float m, float l) {
   const int64_t to = static_cast<int64_t>(at.batch) * p.heads + at.head0 + h;
-  const float lse2 = l == 0.f ? -INFINITY : m + log2f(l);
+  const float lse2 = l == 0.f ? -INFINITY : m + log2f(l * (1.f / RAISED<T>));
   if (p.lse != nullptr) p.lse[to] = lse2 * LN2;
   if (p.logits != nullptr) p.lse2[to] = lse2;
 }
@@ -284,7 +291,7 @@ __device__ void finish(const AttentionParams &p, const Place &at, int pitch, con
         m = top;
       }
       store(h, d, o, l);
-      if (d == 0) tell(p, at, h, m, l);
+      if (d == 0) tell<T>(p, at, h, m, l);
     }
     sm100::cluster_sync_all();   // (no block may leave while another reads its shared memory)
     return;
@@ -353,7 +360,7 @@ __device__ void finish(const AttentionParams &p, const Place &at, int pitch, con
       store(h, d, o, total[R + h]);
     }
   }
-  if (t < at.heads) tell(p, at, t, total[t], total[R + t]);
+  if (t < at.heads) tell<T>(p, at, t, total[t], total[R + t]);
 }
 
 // ---- on CUDA cores: every type, size and alignment -----------------------------------------------------------------------
@@ -464,7 +471,7 @@ __global__ void __launch_bounds__(THREADS) paged_attention_kernel(const Attentio
       for (int o = 8; o > 0; o /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       m = fmaxf(m, top[i]);
       const float safe = m == -INFINITY ? 0.f : m;
-      const float e = exp2f(s - safe), back = exp2f(top[i] - safe);
+      const float e = exp2f(s - safe) * RAISED<T>, back = exp2f(top[i] - safe);
       float l = e;
 #pragma unroll
       for (int o = 8; o > 0; o /= 2) l += __shfl_xor_sync(0xffffffffu, l, o);
@@ -532,7 +539,10 @@ __global__ void __launch_bounds__(THREADS) paged_attention_kernel(const Attentio
 // form takes about 200, and 210 us instead of 165 for two sequences of 120001.)  Every warp has a ring of its own in shared memory that
 // its cp.asyncs fill with CHUNK slots' keys and values at a time, so that no barrier joins warps before the end.  Rows are
 // swizzled in 16-byte words for ldmatrix.  Probabilities are multiplied as two 16-bit values, hi + lo: their sum is the fp32 one to
-// 2^-16 (bf16) or 2^-22, and the second product costs nothing that the memory does not hide.
+// 2^-16, and the second product costs nothing that the memory does not hide.  Two bf16 values are that at any size; two halves only
+// while lo is not cut off at 2^-24, which RAISED keeps true of 24 powers of two below the maximum (16.6 nats).  A chunk with
+// smaller ones among its probabilities, as every one is whose sequence has a slot that outweighs the others by more, multiplies them again,
+// 2^24 times as large (a slot of hardly any weight may still be all there is: the heaviest slot's value may be zero).
 
 template <typename T> struct Mma;
 template <> struct Mma<__half> {
@@ -623,9 +633,10 @@ __device__ __forceinline__ int value_swizzle(int r) {
 
 // HEADS: tiles of 8 query heads.  WHOLE: a chunk of slots lies in one page, and rows have DIM values.
 template <typename T, int DIM, int HEADS, bool WHOLE>
-__global__ void __launch_bounds__(THREADS) paged_attention_mma_kernel(const AttentionParams p) {
+__global__ void __launch_bounds__(THREADS, DIM * sizeof(T) == 128 && HEADS == 2 ? 4 : 0) paged_attention_mma_kernel(const AttentionParams p) {
   using G = Ring<T, DIM>;
-  constexpr bool F32 = sizeof(T) == 4;
+  constexpr bool F32 = sizeof(T) == 4, HALVES = LIFT<T> > 0;
+  constexpr float LEAST = 1.f / 512.f;   // (halves: what is 2^-16 exact as a pair of them)
   constexpr int R = 8 * HEADS, CHUNK = G::CHUNK, STAGES = G::STAGES;
   constexpr int STEPS = G::WORDS / 2, DIM_STEPS = DIM / 16;   // of a product with the keys (two words of a row), with the values
   extern __shared__ __align__(1024) uint8_t ring[];
@@ -879,20 +890,79 @@ __global__ void __launch_bounds__(THREADS) paged_attention_mma_kernel(const Atte
       }
       __syncwarp();
     } else {
-      uint32_t hi[HEADS][2], lo[HEADS][2];
+      // (raised in the exponent: the 2^-20 that this costs them is less than what a pair of 16-bit values does)
+      uint32_t least = 0xffffffffu;   // the smallest probability's bits less one: zeros come last
 #pragma unroll
       for (int t = 0; t < HEADS; ++t) {
-        const float m0 = top[t][0] == -INFINITY ? 0.f : top[t][0], m1 = top[t][1] == -INFINITY ? 0.f : top[t][1];
+        const float m0 = top[t][0] == -INFINITY ? 0.f : top[t][0] - LIFT<T>, m1 = top[t][1] == -INFINITY ? 0.f : top[t][1] - LIFT<T>;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float x = exp2f(s[t][2 * i] - m0), y = exp2f(s[t][2 * i + 1] - m1);
-          sum[t][0] += x;
-          sum[t][1] += y;
-          Mma<T>::split(x, y, hi[t][i], lo[t][i]);
+          s[t][2 * i] = exp2f(s[t][2 * i] - m0);
+          s[t][2 * i + 1] = exp2f(s[t][2 * i + 1] - m1);
+          sum[t][0] += s[t][2 * i];
+          sum[t][1] += s[t][2 * i + 1];
+          if (HALVES) least = min(least, min(__float_as_uint(s[t][2 * i]) - 1u, __float_as_uint(s[t][2 * i + 1]) - 1u));
+        }
+      }
+      if constexpr (HALVES) {
+        if (__any_sync(0xffffffffu, least < __float_as_uint(LEAST) - 1u)) {
+          // those below LEAST by themselves, STEP times as large each time (an fp32 probability is above 2^-149: six times)
+          constexpr float STEP = RAISED<T> / LEAST;
+          float x[HEADS][4], down = 1.f;
+#pragma unroll
+          for (int t = 0; t < HEADS; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              x[t][j] = s[t][j] < LEAST ? s[t][j] : 0.f;
+              s[t][j] = s[t][j] < LEAST ? 0.f : s[t][j];
+            }
+          bool more = true;
+          while (__any_sync(0xffffffffu, more)) {
+            more = false;
+            down *= 1.f / STEP;
+            uint32_t hi[HEADS][2], lo[HEADS][2];
+#pragma unroll
+            for (int t = 0; t < HEADS; ++t)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                float now[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                  float &v = x[t][2 * i + j];
+                  v *= STEP;
+                  now[j] = v < LEAST ? 0.f : v;
+                  v = v < LEAST ? v : 0.f;
+                  more = more || v > 0.f;
+                }
+                Mma<T>::split(now[0], now[1], hi[t][i], lo[t][i]);
+                hi[t][i] = transposed(hi[t][i]);
+                lo[t][i] = transposed(lo[t][i]);
+              }
+#pragma unroll
+            for (int d = 0; d < DIM_STEPS; ++d) {
+              uint32_t a[4];
+              load_matrices<true>(values + value_word[d % 4] + d / 4 * 128, a);
+#pragma unroll
+              for (int t = 0; t < HEADS; ++t) {
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
+                Mma<T>::run(part, a, lo[t][0], lo[t][1]);
+                Mma<T>::run(part, a, hi[t][0], hi[t][1]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[t][d][j] += part[j] * down;
+              }
+            }
+          }
+        }
+      }
+      uint32_t hi[HEADS][2], lo[HEADS][2];
+#pragma unroll
+      for (int t = 0; t < HEADS; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          Mma<T>::split(s[t][2 * i], s[t][2 * i + 1], hi[t][i], lo[t][i]);
           hi[t][i] = transposed(hi[t][i]);
           lo[t][i] = transposed(lo[t][i]);
         }
-      }
 #pragma unroll
       for (int d = 0; d < DIM_STEPS; ++d) {
         uint32_t a[4];
