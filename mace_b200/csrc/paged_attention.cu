@@ -584,6 +584,12 @@ template <> struct Mma<float> {
     hi = (x + 0x1000u) & 0xffffe000u;
     lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
   }
+  // x cut off and what that leaves, 13 bits of which the MMA takes 11: together x to 3 x 2^-23, and never above it, so that the type's
+  // largest values stay finite (what is infinite gives NaN)
+  static __device__ __forceinline__ void cut(uint32_t x, uint32_t &hi, uint32_t &lo) {
+    hi = x & 0xffffe000u;
+    lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
+  }
 };
 
 template <bool TRANS>
@@ -875,7 +881,7 @@ __global__ void __launch_bounds__(THREADS, DIM * sizeof(T) == 128 && HEADS == 2 
             const uint32_t addr = values + half * 8 * G::ROW + ((value_word[i] ^ (d % 2 << 6)) + d / 2 * 128);
             uint32_t x;
             asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(addr) : "memory");
-            Mma<T>::split(x, hi[half][i], lo[half][i]);
+            Mma<T>::cut(x, hi[half][i], lo[half][i]);
           }
         // small products first; what the chunk gives is added to the sum by rounding
 #pragma unroll

@@ -119,3 +119,27 @@ def test_probabilities_of_every_size(ctx, name):
     assert ((out[0].double() - o).abs() <= size * rel + o.abs() * HALF[name]).all()
     assert ((lse[0].double() - l).abs() <= rel + l.abs() * 2.0 ** -22).all()
     assert math.isfinite(float(lse.sum()))
+
+
+def _single(ctx, name, value, length, dim, page):
+    """One slot of a sequence has `value` and -value in turn, the others zeros; logits of zero."""
+    dtype = TYPES[name][1]
+    pages = -(-length // page)
+    k, v = (torch.zeros(pages, 1, page, dim, dtype=dtype) for _ in range(2))
+    at = length // 2
+    v[at // page, 0, at % page] = torch.tensor([value, -value]).repeat(dim // 2).to(dtype)
+    q = torch.ones(1, 4, dim, dtype=dtype)
+    out, _, _ = _run(ctx, name, q, k, v, np.arange(pages, dtype=np.int32)[None], [length], 1.0, page)
+    o = v[at // page, 0, at % page].double() / length
+    # the probability is a quotient of exact numbers: what the product loses of its two factors, the division and the rounding
+    assert ((out[0].double() - o).abs() <= o.abs() * (2.0 ** -20 if name == "f32" else 2.0 ** -16) + o.abs() * HALF[name] * 1.01).all()
+
+
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 20), (256, 16)])
+def test_a_single_value_at_the_types_end(ctx, name, dim, page):
+    """The largest finite values, which the nearest number of fewer bits would make infinite."""
+    top = torch.finfo(TYPES[name][1]).max
+    for value in (top, top * (1 - 2.0 ** -12), top * (1 - 2.0 ** -11), top / 2):
+        for length in (1, 16, 40, 1000):
+            _single(ctx, name, value, length, dim, page)
