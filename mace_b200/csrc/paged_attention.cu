@@ -24,11 +24,13 @@ constexpr int LEAST_RUN = 128;   // slots that are worth a block of their own (1
 constexpr int SCANNED = 1024;    // sequences whose lengths every block reads
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
-// What a probability is multiplied by until the end, relative to one of the running maximum.  Halves reach from 2^-24 to 2^16 only, and
-// most probabilities are small: the largest are brought to their upper end.
-template <typename T> constexpr int LIFT = 0;   // as a power of two
+// What a probability is multiplied by until the end, relative to one of the running maximum, as a power of two.  Halves reach from 2^-24
+// to 2^16 only, and most probabilities are small: the largest are brought to their upper end.  The other types' values may be as large as
+// an fp32 sum can be: probabilities are brought down by so much that 2^24 slots of the maximum's weight sum up to at most one (and
+// what has less than 2^-102 of its weight, e^-70, loses bits, where without the factor it would be 2^-126).
+template <typename T> constexpr int LIFT = -24;
 template <> constexpr int LIFT<__half> = 15;
-template <typename T> constexpr float RAISED = static_cast<float>(1 << LIFT<T>);
+template <typename T> constexpr float RAISED = LIFT<T> < 0 ? 1.f / (1 << -LIFT<T>) : static_cast<float>(1 << (LIFT<T> < 0 ? 0 : LIFT<T>));
 
 struct AttentionParams {
   const void *q, *k, *v;
@@ -860,7 +862,7 @@ __global__ void __launch_bounds__(THREADS, DIM * sizeof(T) == 128 && HEADS == 2 
       const float m0 = top[0][0] == -INFINITY ? 0.f : top[0][0], m1 = top[0][1] == -INFINITY ? 0.f : top[0][1];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float x = exp2f(s[0][2 * i] - m0), y = exp2f(s[0][2 * i + 1] - m1);
+        const float x = exp2f(s[0][2 * i] - m0) * RAISED<T>, y = exp2f(s[0][2 * i + 1] - m1) * RAISED<T>;
         sum[0][0] += x;
         sum[0][1] += y;
         *reinterpret_cast<float2 *>(&weight_s[warp][row + 8 * i][2 * pair]) = make_float2(x, y);

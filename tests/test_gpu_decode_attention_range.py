@@ -143,3 +143,39 @@ def test_a_single_value_at_the_types_end(ctx, name, dim, page):
     for value in (top, top * (1 - 2.0 ** -12), top * (1 - 2.0 ** -11), top / 2):
         for length in (1, 16, 40, 1000):
             _single(ctx, name, value, length, dim, page)
+
+
+def _even(ctx, name, values, length, heads, kv_heads, dim, page, tensor_cores=True):
+    """Every slot has the same logit: the result is the values' mean, whatever their sum would be."""
+    dtype = TYPES[name][1]
+    pages = -(-length // page)
+    k = torch.zeros(pages, kv_heads, page, dim, dtype=dtype)
+    v = values(pages * page).to(dtype)[:, None, None].expand(-1, kv_heads, dim).reshape(pages, page, kv_heads, dim).transpose(1, 2).contiguous()
+    q = torch.ones(1, heads, dim, dtype=dtype)
+    ctx.set_option("tensor_cores", int(tensor_cores))
+    try:
+        out, lse, _ = _run(ctx, name, q, k, v, np.arange(pages, dtype=np.int32)[None], [length], 1.0, page)
+    finally:
+        ctx.set_option("tensor_cores", 1)
+    rows = v.transpose(1, 2).reshape(-1, kv_heads, dim)[:length].double()
+    o, size = rows.mean(0)[0, 0], rows.abs().mean(0)[0, 0]
+    # probabilities are a power of two; sums over slots as ever, of products that lose 2^-20 or nothing
+    assert ((out.double() - o).abs() <= size * ((length / 4 + 150) * 2.0 ** -23 + 2.0 ** -20) + o.abs() * HALF[name] * 1.01).all()
+    assert ((lse.double() - math.log(length)).abs() <= 2.0 ** -20).all()
+
+
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("length", [2, 17, 300, 9000, 60000])
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(8, 2, 128, 16), (24, 1, 64, 20), (1, 1, 256, 16), (3, 3, 50, 7)])
+def test_values_whose_sum_no_float_holds(ctx, name, length, heads, kv_heads, dim, page):
+    """All values are near the type's largest, of one sign and of both."""
+    top = float(torch.finfo(TYPES[name][1]).max)
+    _even(ctx, name, lambda n: torch.full((n,), top * 0.99), length, heads, kv_heads, dim, page)
+    _even(ctx, name, lambda n: torch.full((n,), top * 0.99).where(torch.arange(n) % 3 > 0, torch.tensor(-top)), length, heads, kv_heads, dim, page)
+
+
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+def test_values_whose_sum_no_float_holds_on_cuda_cores(ctx, name):
+    top = float(torch.finfo(TYPES[name][1]).max)
+    for length in (2, 300, 9000):
+        _even(ctx, name, lambda n: torch.full((n,), top * 0.99), length, 8, 2, 128, 16, tensor_cores=False)
