@@ -379,7 +379,7 @@ bool conv_map_possible(const mb_context *ctx, const mb_cut_gemm &g) {
 // GPC, and not every GPC has a whole number of clusters' SMs).
 int64_t mb_resident_cluster_ctas(mb_context *ctx, int s) {
   if (s == 1) return ctx->num_sms;
-  const int slot = s == 2 ? 1 : s == 4 ? 2 : 3;
+  const int slot = s == 2 ? 1 : s == 4 ? 2 : s == 8 ? 3 : 0;   // (0: clusters of 16)
   if (ctx->cut_clusters[slot] == 0) {
     using C = Cfg<128, false, 128, 1>;
     auto kern = gemm_u8_cut_kernel<128, A_KMAJOR, false, 128, 1>;
@@ -396,6 +396,7 @@ int64_t mb_resident_cluster_ctas(mb_context *ctx, int s) {
     probe.numAttrs = 1;
     int n = 0;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES) != cudaSuccess ||
+        (s > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) ||
         cudaOccupancyMaxActiveClusters(&n, kern, &probe) != cudaSuccess || n < 1) {
       cudaGetLastError();
       n = std::max(1, (ctx->num_sms - 20) / s);

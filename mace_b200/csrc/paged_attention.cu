@@ -20,7 +20,7 @@ namespace {
 constexpr int THREADS = 128;
 constexpr int WARPS = THREADS / 32;
 constexpr int MAX_SPLITS = 128;
-constexpr int LEAST_RUN = 128;   // slots that are worth a block of their own (1000 slots, 8 heads: 64 12.2 us, 128 10.8, 256 13.7)
+constexpr int LEAST_RUN = kv::LEAST_RUN;
 constexpr int SCANNED = 1024;    // sequences whose lengths every block reads
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
@@ -1131,14 +1131,17 @@ extern "C" int mb_paged_attention(mb_context *ctx, const void *q, const void *k_
   p.batch = static_cast<int>(batch);
   p.pitch = static_cast<int>(align_up(p.dim, 4));
   const int64_t units = batch * kv_heads * p.blocks;
-  // Work that is over before its blocks' parts could meet in memory: each head's slots over a cluster, 128 of them a block at least
-  // (1000 slots, 8 heads: 10.4 us with the runs joined by the last block, 7.7 on clusters of 8; 8192: 18.6 and 16.1 on 16).
-  constexpr int64_t SMALL = 64ll << 20;
-  const int most = by_mma ? 16 : 8;
-  p.cluster = 1;
-  if (units * p.longest * 2 * head_dim * kv::type_bytes(dtype) <= SMALL)
-    while (p.cluster < most && units * p.cluster * 2 <= 2 * ctx->num_sms && p.longest > LEAST_RUN * p.cluster) p.cluster *= 2;
   const int per_sm = three ? 2 : !by_mma ? (rows * p.dim >= 1024 ? 3 : 5) : p.dim * kv::type_bytes(dtype) > 256 ? 1 : p.dim * kv::type_bytes(dtype) > 128 ? 3 : 4;
+  // Small work: each head's slots over a cluster, which joins without memory.  What a block of one can be given: 1024 slots of 16-bit
+  // types on the tensor cores, 512 of fp32 ones up to 64, 256 up to 128, and 128 on CUDA cores, whose clusters are of 8 (one head of 128, bf16, on clusters
+  // and as runs: 1000 slots 7.0 and 9.4 us, 16000 21.2 and 25.3, 32000 34.1 and 27.1; fp32 4000 15.7 and 15.4, 8000 23.7 and 19.6; fp32 of 256,
+  // CUDA cores, 1000 26.4 and 28.3, 2000 70.7 and 43.2).  All of a launch's are resident at once: where a block fills an SM, as many as
+  // the device's clusters of one CTA an SM (8 heads of 256, 2000 slots, on 128 CTAs in clusters of 16, of which 112 are resident: 20.8 us,
+  // as runs 16.2).
+  int64_t room_for[5];
+  for (int i = 0; i < 5; ++i) room_for[i] = per_sm > 1 ? 2 * ctx->num_sms : mb_resident_cluster_ctas(ctx, 1 << i);
+  const int share = !by_mma ? 128 : !f32 ? 1024 : head_dim <= 64 ? 512 : 256;
+  p.cluster = kv::cluster_of(units, p.longest, 2 * head_dim * kv::type_bytes(dtype), by_mma ? 16 : 8, share, room_for);
   // The runs wanted of all heads together: one round of resident blocks where the heads leave room for it, less one for each head, whose
   // last run is not a whole one; else half as many again as are resident.  (256 heads of 4096 slots, 444 blocks resident: 444 wanted
   // 105 us, 666 90, 888 97; 512 ragged ones of up to 8192: 168, 164, 164.  As many as fill the last round, up to 8 of them: 94 and 173.)

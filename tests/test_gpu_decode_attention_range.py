@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from decode_ref import HALF, TINY, TYPES, Values, attend
+from test_gpu_decode_attention import Case
 
 pytestmark = pytest.mark.gpu
 
@@ -179,3 +180,12 @@ def test_values_whose_sum_no_float_holds_on_cuda_cores(ctx, name):
     top = float(torch.finfo(TYPES[name][1]).max)
     for length in (2, 300, 9000):
         _even(ctx, name, lambda n: torch.full((n,), top * 0.99), length, 8, 2, 128, 16, tensor_cores=False)
+
+
+@pytest.mark.parametrize("name,heads,kv_heads,dim,page", [("bf16", 8, 1, 128, 16), ("f16", 8, 2, 64, 16), ("f32", 4, 1, 128, 16), ("f32", 4, 2, 64, 20),
+                                                          ("f32", 4, 1, 256, 16), ("bf16", 16, 8, 256, 16), ("bf16", 4, 1, 50, 16)])
+@pytest.mark.parametrize("length", [1000, 1025, 2048, 4097, 9000, 17000, 40000])
+def test_few_heads_and_long_sequences(ctx, name, heads, kv_heads, dim, page, length):
+    """Either side of where a head's slots outgrow a cluster, with and without weights."""
+    for weights in (False, True):
+        Case(ctx, name, [length], heads, kv_heads, dim, page, seed=length, weights=weights).run().check()
