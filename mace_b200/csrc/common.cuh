@@ -156,6 +156,9 @@ int mb_op_counters(mb_context *ctx, size_t count, unsigned **ptr);
 // predecessor has completed and its writes are visible.  mb_grid_dep_launch(), called at the top
 // of a kernel, lets the kernel BEHIND it do the same.  Kernels launched the ordinary way are
 // full barriers in the stream, so the two kinds mix freely.
+// A kernel that takes tensor memory calls it behind its allocation: the one behind it, once
+// started, allocates before it waits.  Were it first on an SM, an allocation here that finds no
+// room would wait for columns that are given back only when this kernel has ended.
 __device__ __forceinline__ void mb_grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void mb_grid_dep_launch() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

@@ -165,7 +165,6 @@ conv_f32_direct_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_c
   const uint32_t w_row_bytes = p.KW * C::W_BYTES, w_stages = p.w_stages;
   const uint32_t w_base = smem_base + 1024, patch0 = w_base + w_stages * w_row_bytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  mb_grid_dep_launch();
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map_w);
     for (int s = 0; s < MAX_W_STAGES; ++s) {
@@ -188,6 +187,7 @@ conv_f32_direct_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_c
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
     tmem_relinquish();
+    mb_grid_dep_launch();  // (behind the allocation: common.cuh says why)
   }
   auto fail = [&](int code) {
     *abort_flag = 1;

@@ -100,7 +100,6 @@ __global__ void __launch_bounds__(THREADS, 1) conv_f32_stem_kernel(const __grid_
   uint8_t *w_smem = smem + HEAD;
   const uint32_t w_base = smem_base + HEAD;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  mb_grid_dep_launch();
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.slots; ++s) {
       mbar_init(full_bar + 8 * s, IN_WARPS);
@@ -121,6 +120,7 @@ __global__ void __launch_bounds__(THREADS, 1) conv_f32_stem_kernel(const __grid_
   if (warp == MMA_WARP) {
     tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
     tmem_relinquish();
+    mb_grid_dep_launch();  // (behind the allocation: common.cuh says why)
   }
   if (threadIdx.x < BN) table[threadIdx.x] = make_float2(0.f, 0.f);
   for (int i = threadIdx.x; i < p.KH * MM * W_MMA / 16; i += THREADS) reinterpret_cast<uint4 *>(w_smem)[i] = make_uint4(0, 0, 0, 0);

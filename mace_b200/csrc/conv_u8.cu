@@ -355,7 +355,6 @@ __global__ void __launch_bounds__(128, 8) conv_u8_stem_mma_kernel(const Params q
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bar + 1);
   const uint32_t mma_bar = smem_u32(bar);
   const int warp = threadIdx.x >> 5;
-  mb_grid_dep_launch();
   if (threadIdx.x == 0) {
     mbar_init(mma_bar, 1);
     fence_barrier_init();
@@ -363,6 +362,7 @@ __global__ void __launch_bounds__(128, 8) conv_u8_stem_mma_kernel(const Params q
   if (warp == 0) {
     tmem_alloc(smem_u32(tmem_slot), static_cast<uint32_t>(q.acc_cols));
     tmem_relinquish();
+    mb_grid_dep_launch();  // (behind the allocation: common.cuh says why)
   }
   if (!q.filter_const) mb_grid_dep_wait();
   // B: row o = the filter row (KD bytes, zero tail); byte k of row n lives at [k / 16][n][k % 16].

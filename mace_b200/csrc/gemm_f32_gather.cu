@@ -219,7 +219,6 @@ gemm_f32_gather_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_c
   volatile int *again = abort_flag + 1;  // a result is not finite
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr uint32_t half = MODE != WHOLE ? 0x1000u : 0u;
-  mb_grid_dep_launch();
 
   if (threadIdx.x == MMA_WARP * 32) {
     for (int s = 0; s < STAGES; ++s) {
@@ -239,6 +238,7 @@ gemm_f32_gather_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_c
   if (warp == FIRST_E) {
     tmem_alloc(smem_u32(tmem_slot), 512);
     tmem_relinquish();
+    mb_grid_dep_launch();  // (behind the allocation: common.cuh says why)
   }
   const int rank = p.splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int kb_begin = static_cast<int>(static_cast<int64_t>(p.k_blocks) * rank / p.splits);

@@ -725,7 +725,6 @@ gemm_f32_pairs_kernel(const __grid_constant__ CUtensorMap tmap_x,
   const FShared<BN> sh(smem_raw);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  mb_grid_dep_launch();  // the kernel behind this one may start its own prologue
 
   if (threadIdx.x == 0) {
     prefetch_tensormap(&tmap_x);
@@ -740,6 +739,7 @@ gemm_f32_pairs_kernel(const __grid_constant__ CUtensorMap tmap_x,
     tmem_alloc(smem_u32(sh.tmem_slot), Cfg::TMEM_COLS);
     tmem_relinquish();
     for (int i = lane; i < 2 * MARKS; i += 32) sh.marks[i] = 0;
+    mb_grid_dep_launch();  // (behind the allocation: common.cuh says why)
   }
   tc_fence_before_sync();
   __syncthreads();

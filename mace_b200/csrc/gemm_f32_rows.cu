@@ -95,7 +95,6 @@ gemm_f32_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
   volatile int *again = abort_flag + 1;
   float *unscales = reinterpret_cast<float *>(smem + C::SCALE_AT);  // [SCALE_SLOTS][ROWS]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  mb_grid_dep_launch();
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map_x);
     prefetch_tensormap(&map_w);
@@ -115,6 +114,7 @@ gemm_f32_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
     tmem_relinquish();
+    mb_grid_dep_launch();  // (behind the allocation: common.cuh says why)
   }
   auto fail = [&](int code) {
     *abort_flag = 1;

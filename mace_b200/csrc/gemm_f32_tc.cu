@@ -168,7 +168,6 @@ gemm_f32_tc_kernel(const __grid_constant__ CUtensorMap tmap_x,
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  mb_grid_dep_launch();  // the kernel behind this one may start its own prologue
 
   if (threadIdx.x == 0) {
     prefetch_tensormap(&tmap_x);
@@ -189,6 +188,7 @@ gemm_f32_tc_kernel(const __grid_constant__ CUtensorMap tmap_x,
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), Cfg::TMEM_COLS);
     tmem_relinquish();
+    mb_grid_dep_launch();  // (behind the allocation: common.cuh says why)
   }
   tc_fence_before_sync();
   __syncthreads();

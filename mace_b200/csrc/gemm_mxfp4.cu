@@ -139,7 +139,6 @@ gemm_mxfp4_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + C::RING + 16 * STAGES + 16 * C::ACCUMULATORS);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  mb_grid_dep_launch();
 
   if (threadIdx.x == MMA_WARP * 32) {
     prefetch_tensormap(&map_a);
@@ -158,6 +157,7 @@ gemm_mxfp4_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
   if (warp == TMA_WARP) {
     tmem_alloc(smem_u32(tmem_slot), C::TMEM);
     tmem_relinquish();
+    mb_grid_dep_launch();  // (behind the allocation: common.cuh says why)
   }
   // this CTA's tiles, and its run of their depth
   const int rank = p.splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;

@@ -127,7 +127,6 @@ gemm_u8_cut_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool patch = A_KIND == A_CONV && p.patch;
   const bool want_a = p.tail.zp_b != 0, want_b = p.tail.zp_a != 0;
-  mb_grid_dep_launch();
 
   if (threadIdx.x == MMA_WARP * 32) {
     prefetch_tensormap(&map_a);
@@ -145,6 +144,7 @@ gemm_u8_cut_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   if (warp == TMA_WARP) {
     tmem_alloc(smem_u32(tmem_slot), BN);
     tmem_relinquish();
+    mb_grid_dep_launch();  // (behind the allocation: common.cuh says why)
   }
   for (int i = threadIdx.x; i < 128 + BN; i += THREADS) row_sums[i] = 0;
 

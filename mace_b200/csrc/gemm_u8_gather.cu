@@ -201,7 +201,6 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_u8_gather_kernel(const __grid
   uint32_t *row_sums = reinterpret_cast<uint32_t *>(smem + C::RING + 256);  // [128]
   uint32_t *col_sums = row_sums + 128;                                      // [BN]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  mb_grid_dep_launch();
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -215,6 +214,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_u8_gather_kernel(const __grid
   if (warp == LOAD_WARPS) {
     tmem_alloc(smem_u32(tmem_slot), BN);
     tmem_relinquish();
+    mb_grid_dep_launch();  // (behind the allocation: common.cuh says why)
   }
   for (int i = threadIdx.x; i < 128 + BN; i += THREADS) row_sums[i] = 0;
 

@@ -393,7 +393,6 @@ gemm_u8_tc_kernel(const __grid_constant__ CUtensorMap tmap_a,
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  mb_grid_dep_launch();  // the kernel behind this one may start its own prologue
 
   if (threadIdx.x == 0) {
     MB_STAMP(0);
@@ -423,6 +422,7 @@ gemm_u8_tc_kernel(const __grid_constant__ CUtensorMap tmap_a,
       tmem_alloc(smem_u32(tmem_slot), Cfg::TMEM_COLS);
       tmem_relinquish();
     }
+    mb_grid_dep_launch();  // (behind the allocation: common.cuh says why)
   }
   if (TCR) {
     // the 16 rows of ones behind every stage's B tile (TMA never writes there)
