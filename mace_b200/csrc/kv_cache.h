@@ -50,6 +50,9 @@ inline int cluster_of(int64_t units, int64_t longest, int64_t slot_bytes, int mo
   return longest > share * blocks ? 1 : blocks;
 }
 
+// Slots of a sequence that a block of the second kernel of attention with weights has.
+constexpr int WEIGHT_SLOTS = 1024;
+
 // What a check of arguments says: code MB_SUCCESS, or the status to return and why.
 struct Verdict {
   int code;
@@ -177,6 +180,9 @@ inline Verdict check_attention(const void *q, const void *k_cache, const void *v
   KV_REQUIRE(weights_in == nullptr || weights_out != nullptr, "weights_in without weights_out");
   KV_REQUIRE(weights_out == nullptr || (weights_stride >= longest_of(max_length, max_pages, page_size) && weights_stride <= MOST),
              "weights_stride below the longest sequence, or too large");
+  if (weights_out != nullptr &&
+      batch * kv_heads * ((longest_of(max_length, max_pages, page_size) + static_cast<int64_t>(WEIGHT_SLOTS) - 1) / WEIGHT_SLOTS) > MOST)
+    return unsupported("too many slots");
   if (batch == 0) return fine();
   KV_REQUIRE(q != nullptr && out != nullptr && lengths != nullptr && (max_pages == 0 || table != nullptr) &&
              (num_pages == 0 || (k_cache != nullptr && v_cache != nullptr)), "null operand");

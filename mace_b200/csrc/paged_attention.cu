@@ -1044,15 +1044,13 @@ int launch_mma(mb_context *ctx, const AttentionParams &p, unsigned grid, int row
   return MB_SUCCESS;
 }
 
-// What each slot has received of the query heads' probabilities, on top of what it had.  Four slots a thread: a word of every head's
-// logits, all in flight together.
-constexpr int WEIGHT_SLOTS = 1024;   // of a block
-
+// What each slot has received of the query heads' probabilities, on top of what it had.  Four slots a thread (kv::WEIGHT_SLOTS a block): a
+// word of every head's logits, all in flight together.
 __global__ void __launch_bounds__(256) attention_weights_kernel(const AttentionParams p, int chunks) {
   mb_grid_dep_launch();
   mb_grid_dep_wait();
   const int unit = blockIdx.x / chunks, batch = unit / p.kv_heads, kv_head = unit % p.kv_heads;
-  const int slot = (blockIdx.x % chunks) * WEIGHT_SLOTS + threadIdx.x * 4;
+  const int slot = (blockIdx.x % chunks) * kv::WEIGHT_SLOTS + threadIdx.x * 4;
   bool bad;
   const int length = kv::usable_length(mb_load(p.lengths + batch), p.longest, &bad);
   if (slot >= length) return;
@@ -1193,8 +1191,7 @@ extern "C" int mb_paged_attention(mb_context *ctx, const void *q, const void *k_
   MB_CUDA(ctx, e);
   ctx->launches++;
   if (logits > 0) {
-    const int chunks = (p.longest + WEIGHT_SLOTS - 1) / WEIGHT_SLOTS;
-    if (batch * kv_heads * chunks > kv::MOST) return mb_fail(ctx, MB_UNSUPPORTED, "mb_paged_attention: too many slots");
+    const int chunks = (p.longest + kv::WEIGHT_SLOTS - 1) / kv::WEIGHT_SLOTS;
     MB_CUDA(ctx, mb_launch_chained(ctx, attention_weights_kernel, dim3(static_cast<unsigned>(batch * kv_heads * chunks)), dim3(256), 0, p, chunks));
     ctx->launches++;
   }

@@ -42,8 +42,28 @@ static void clusters() {
   EXPECT(kv::cluster_of(8, 2000, 1024, 16, 1024, room) == 8);
 }
 
+alignas(16) static char memory[64];
+static const void *const X = memory;
+static void *const Y = memory + 32;
+static const int32_t *const I = reinterpret_cast<const int32_t *>(memory);
+static float *const F = reinterpret_cast<float *>(memory);
+
+// What attention with weights would refuse after its first kernel is refused before it.
+static void weights_of_too_many_slots() {
+  const auto code = [](int64_t batch, int64_t kv_heads, int64_t length, float *weights) {
+    return kv::check_attention(X, X, X, I, I, Y, nullptr, nullptr, weights, batch, kv_heads, kv_heads, 8, kv_heads * 8, kv_heads * 8, 1 << 20, 16,
+                               1 << 26, length, 0, length, MB_F16).code;
+  };
+  EXPECT(code(1 << 15, 1 << 8, 256 * 1024, F) == MB_UNSUPPORTED);
+  EXPECT(code(1 << 15, 1 << 8, 255 * 1024, F) == MB_SUCCESS);
+  EXPECT(code(1 << 15, 1 << 8, 255 * 1024 + 1, F) == MB_UNSUPPORTED);
+  EXPECT(code(1 << 15, 1 << 8, 256 * 1024, nullptr) == MB_SUCCESS);
+  EXPECT(code(0, 1 << 8, 256 * 1024, F) == MB_SUCCESS);
+}
+
 int main() {
   clusters();
+  weights_of_too_many_slots();
   if (failures != 0) std::printf("%d failures\n", failures);
   return failures != 0;
 }
