@@ -192,6 +192,21 @@ inline Verdict check_attention(const void *q, const void *k_cache, const void *v
   return fine();
 }
 
+// How eviction copies rows of `row_bytes`: in words of `word` bytes, as wide as every address in `bits` (which has the row's bytes
+// among its own) allows, whole rows of at most COPY_WORDS words to a block.
+constexpr int COPY_WORDS = 512;
+struct CopyShape {
+  int64_t word, words, rows;   // rows: of a block, 0 where not one fits
+};
+inline CopyShape copy_shape(uintptr_t bits, int64_t row_bytes) {
+  const int64_t word = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 2;
+  return {word, row_bytes / word, COPY_WORDS / (row_bytes / word)};
+}
+inline uintptr_t copy_bits(const void *k_src, const void *v_src, const void *k_dst, const void *v_dst, int64_t row_bytes) {
+  return reinterpret_cast<uintptr_t>(k_src) | reinterpret_cast<uintptr_t>(v_src) | reinterpret_cast<uintptr_t>(k_dst) |
+         reinterpret_cast<uintptr_t>(v_dst) | static_cast<uintptr_t>(row_bytes);
+}
+
 inline Verdict check_evict(const void *k_src, const void *v_src, const int32_t *src_table, const int32_t *lengths, const float *weights,
                            const void *k_dst, const void *v_dst, const int32_t *dst_table, const int32_t *dst_lengths,
                            const float *dst_weights, const int32_t *kept, int64_t batch, int64_t kv_heads, int64_t dim,
@@ -222,6 +237,10 @@ inline Verdict check_evict(const void *k_src, const void *v_src, const int32_t *
              aligned(dst_table, 4) && aligned(lengths, 4) && aligned(dst_lengths, 4) && aligned(weights, 4) &&
              aligned(dst_weights, 4) && aligned(kept, 4), "misaligned operand");
   KV_REQUIRE(apart(weights, batch * kv_heads * weights_stride, dst_weights, batch * kv_heads * dst_weights_stride), "dst_weights may not lie in weights");
+  const int64_t row_bytes = dim * type_bytes(dtype);
+  const CopyShape copy = copy_shape(copy_bits(k_src, v_src, k_dst, v_dst, row_bytes), row_bytes);
+  if (copy.rows == 0) return unsupported("head_dim too large");
+  if (batch * kv_heads * (((stays < 1 ? 1 : stays) + copy.rows - 1) / copy.rows) > MOST) return unsupported("too many slots");
   return fine();
 }
 

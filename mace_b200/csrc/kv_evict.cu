@@ -312,14 +312,13 @@ __global__ void __launch_bounds__(COPY_THREADS) evict_copy_kernel(const EvictPar
   }
 }
 
+static_assert(COPY_THREADS * COPY_EACH == kv::COPY_WORDS, "words of a block");
+
 template <typename Word>
-int launch_copy(mb_context *ctx, EvictParams &p, int64_t units, int64_t row_bytes, bool clear) {
-  const int64_t words = row_bytes / sizeof(Word);
-  if (words > COPY_THREADS * COPY_EACH) return mb_fail(ctx, MB_UNSUPPORTED, "mb_kv_evict: head_dim too large");
-  p.words = static_cast<int>(words);
+int launch_copy(mb_context *ctx, EvictParams &p, int64_t units, const kv::CopyShape &copy, bool clear) {
+  p.words = static_cast<int>(copy.words);
   fast_div_make(p.words, &p.word_mul, &p.word_shift);
-  p.chunks = static_cast<int>(ceil_div64(std::min(p.budget, std::max(p.longest, 1)), COPY_THREADS * COPY_EACH / p.words));
-  if (units * p.chunks > kv::MOST) return mb_fail(ctx, MB_UNSUPPORTED, "mb_kv_evict: too many slots");
+  p.chunks = static_cast<int>(ceil_div64(std::min(p.budget, std::max(p.longest, 1)), copy.rows));
   MB_CUDA(ctx, mb_launch_chained(ctx, clear ? evict_copy_kernel<Word, true> : evict_copy_kernel<Word, false>, dim3(static_cast<unsigned>(units * p.chunks)), dim3(COPY_THREADS), 0, p));
   ctx->launches++;
   return MB_SUCCESS;
@@ -350,12 +349,8 @@ int evict(mb_context *ctx, const char *who, const void *k_src, const void *v_src
   fast_div_make(static_cast<uint32_t>(page_size), &p.page_mul, &p.page_shift);
   p.status = ctx->dev_status;
 
-  // the widest word that a row and the four pools are made of
   const int64_t units = batch * kv_heads, row_bytes = head_dim * kv::type_bytes(dtype);
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(k_src) | reinterpret_cast<uintptr_t>(v_src) | reinterpret_cast<uintptr_t>(k_dst) |
-                         reinterpret_cast<uintptr_t>(v_dst) | static_cast<uintptr_t>(row_bytes);
-  if (row_bytes / (bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 2) > COPY_THREADS * COPY_EACH)
-    return mb_fail(ctx, MB_UNSUPPORTED, "mb_kv_evict: head_dim too large");
+  const kv::CopyShape copy = kv::copy_shape(kv::copy_bits(k_src, v_src, k_dst, v_dst, row_bytes), row_bytes);
   // A CTA of 1024 threads an SM, or, where there are more heads than SMs, two of 512; 4096 weights or more to each of a cluster.
   // (16 sequences of 8192, 8 heads: two CTAs of 512 a head 17.7 us, one of 1024 14.7.)
   constexpr int MOST_KEYS = 20 << 10;
@@ -365,7 +360,6 @@ int evict(mb_context *ctx, const char *who, const void *k_src, const void *v_src
   while (p.cluster < 16 && p.longest > MOST_KEYS * p.cluster) p.cluster *= 2;
   const int64_t keys = ceil_div64(p.longest, p.cluster);
   p.cached = keys <= MOST_KEYS;
-  if (units * p.cluster > kv::MOST) return mb_fail(ctx, MB_UNSUPPORTED, "mb_kv_evict: too many kv heads");
   if (!ctx->evict_attr_set) {
     for (const auto kern : {evict_select_kernel<512>, evict_select_kernel<1024>}) {
       MB_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_KEYS * 4));
@@ -376,9 +370,9 @@ int evict(mb_context *ctx, const char *who, const void *k_src, const void *v_src
   MB_CUDA(ctx, mb_launch_clusters(ctx, large ? evict_select_kernel<1024> : evict_select_kernel<512>, static_cast<unsigned>(units * p.cluster),
                                   large ? 1024 : 512, p.cached ? static_cast<size_t>(keys) * 4 : 0, p.cluster, p));
   ctx->launches++;
-  if (bits % 16 == 0) return launch_copy<uint4>(ctx, p, units, row_bytes, clear);
-  if (bits % 4 == 0) return launch_copy<uint32_t>(ctx, p, units, row_bytes, clear);
-  return launch_copy<uint16_t>(ctx, p, units, row_bytes, clear);
+  if (copy.word == 16) return launch_copy<uint4>(ctx, p, units, copy, clear);
+  if (copy.word == 4) return launch_copy<uint32_t>(ctx, p, units, copy, clear);
+  return launch_copy<uint16_t>(ctx, p, units, copy, clear);
 }
 
 }  // namespace

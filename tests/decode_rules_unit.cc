@@ -61,9 +61,32 @@ static void weights_of_too_many_slots() {
   EXPECT(code(0, 1 << 8, 256 * 1024, F) == MB_SUCCESS);
 }
 
+// What eviction would refuse between its two kernels is refused before the first.
+static void rows_too_many_or_too_long() {
+  const auto code = [](int64_t batch, int64_t dim, int64_t budget, const void *k) {
+    return kv::check_evict(k, X, I, I, F, Y, Y, I, I, F + 16, I, batch, 1, dim, 16, 1 << 20, 1 << 20, 1 << 20, 1 << 20, budget, budget, budget, 0, 0,
+                           MB_F32, budget).code;
+  };
+  // (weights that overlap would be refused first: 2^18 rows of 2^14 lie 2^32 values apart)
+  const auto far = [&](int64_t batch, int64_t dim, int64_t budget, const void *k) {
+    return kv::check_evict(k, X, I, I, F, Y, Y, I, I, reinterpret_cast<const float *>(uintptr_t{1} << 45), I, batch, 1, dim, 16, 1 << 20, 1 << 20, 1 << 20,
+                           1 << 20, budget, budget, budget, 0, 0, MB_F32, budget).code;
+  };
+  EXPECT(far(1 << 18, 2048, 1 << 13, X) == MB_UNSUPPORTED);   // a row to a block, 2^31 of them
+  EXPECT(far(1 << 18, 2048, (1 << 13) - 1, X) == MB_SUCCESS);
+  EXPECT(far(1 << 18, 1024, 1 << 13, X) == MB_SUCCESS);
+  EXPECT(far(1 << 18, 128, 1 << 13, memory + 4) == MB_SUCCESS);
+  EXPECT(far(1 << 18, 512, 1 << 13, memory + 4) == MB_UNSUPPORTED);   // words of 4 bytes: as many blocks as of 2048 above
+  EXPECT(code(1, 2048, 1, X) == MB_SUCCESS);
+  EXPECT(code(1, 2052, 1, X) == MB_UNSUPPORTED);
+  EXPECT(code(1, 512, 1, memory + 4) == MB_SUCCESS);
+  EXPECT(code(1, 513, 1, memory + 4) == MB_UNSUPPORTED);
+}
+
 int main() {
   clusters();
   weights_of_too_many_slots();
+  rows_too_many_or_too_long();
   if (failures != 0) std::printf("%d failures\n", failures);
   return failures != 0;
 }
