@@ -66,10 +66,10 @@ inline bool is_type(int dtype) { return dtype == MB_F32 || dtype == MB_F16 || dt
 inline int type_bytes(int dtype) { return dtype == MB_F32 ? 4 : 2; }
 inline bool aligned(const void *p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
-// Extents above these are refused, so that counts fit 31 bits and byte offsets 63.
+// Extents above these are refused, so that counts fit 31 bits and byte offsets 63 (a tensor's two strides together).
 constexpr int64_t MOST = INT32_MAX;
 constexpr int64_t MOST_DIM = 1 << 16;   // rotary head_dim
-constexpr int64_t MOST_STRIDE = 1ll << 40;
+constexpr int64_t MOST_STRIDE = 1ll << 40, MOST_OFFSET = 1ll << 59;
 
 #define KV_REQUIRE(cond, why) \
   do {                        \
@@ -89,20 +89,29 @@ inline Verdict check_rotary(int64_t dim, int64_t rotary, int64_t tokens, int64_t
   return fine();
 }
 
-inline Verdict check_stride(int64_t stride) {
-  KV_REQUIRE(stride >= 0 && stride <= MOST_STRIDE, "stride is negative or too large");
+// Whether the last of `count` rows `stride` apart has a place.
+inline bool reaches(int64_t count, int64_t stride) { return count <= 1 || stride == 0 || count - 1 <= MOST_OFFSET / stride; }
+
+inline Verdict check_stride(int64_t stride, int64_t count) {
+  KV_REQUIRE(stride >= 0 && stride <= MOST_STRIDE && reaches(count, stride), "stride is negative or too large");
   return fine();
+}
+
+// outer >= (count - 1) * step + width, however large they are.
+inline bool holds(int64_t outer, int64_t count, int64_t step, int64_t width) {
+  return outer >= width && (count <= 1 || step == 0 || (outer - width) / step >= count - 1);
 }
 
 // Rows of `width` elements, `count` of them, in a buffer that is written: they may not overlap.
 inline Verdict check_rows(int64_t count, int64_t stride, int64_t width) {
-  KV_REQUIRE(stride >= 0 && stride <= MOST_STRIDE && (count <= 1 || stride >= width), "output rows overlap, or stride is too large");
+  KV_REQUIRE(stride >= 0 && stride <= MOST_STRIDE && reaches(count, stride) && (count <= 1 || stride >= width), "output rows overlap, or stride is too large");
   return fine();
 }
 
 inline Verdict check_pool(int64_t num_pages, int64_t page_size, int64_t kv_heads, int64_t dim) {
   KV_REQUIRE(num_pages >= 0 && page_size >= 1, "bad number or size of pages");
   if (page_size > MOST || num_pages > MOST / page_size || kv_heads * dim > MOST) return unsupported("more than 2^31 - 1 slots");
+  if (num_pages * page_size > MOST_OFFSET / (kv_heads * dim)) return unsupported("pool too large");
   return fine();
 }
 
@@ -123,12 +132,13 @@ inline Verdict check_rope(const void *x, const void *y, const int32_t *positions
                           int64_t y_head, int dtype) {
   KV_PASS(check_heads(tokens, heads, dim, dtype));
   KV_PASS(check_rotary(dim, rotary, tokens, heads));
-  KV_PASS(check_stride(x_token));
-  KV_PASS(check_stride(x_head));
-  KV_REQUIRE(y_token >= 0 && y_head >= 0 && y_token <= MOST_STRIDE && y_head <= MOST_STRIDE, "stride is negative or too large");
+  KV_PASS(check_stride(x_token, tokens));
+  KV_PASS(check_stride(x_head, heads));
+  KV_PASS(check_stride(y_token, tokens));
+  KV_PASS(check_stride(y_head, heads));
   // rows of heads inside tokens or of tokens inside heads
-  const bool inside = (heads <= 1 || y_head >= dim) && (tokens <= 1 || y_token >= (heads - 1) * y_head + dim);
-  const bool outside = (tokens <= 1 || y_token >= dim) && (heads <= 1 || y_head >= (tokens - 1) * y_token + dim);
+  const bool inside = (heads <= 1 || y_head >= dim) && (tokens <= 1 || holds(y_token, heads, y_head, dim));
+  const bool outside = (tokens <= 1 || y_token >= dim) && (heads <= 1 || holds(y_head, tokens, y_token, dim));
   KV_REQUIRE(inside || outside, "output heads overlap");
   if (tokens == 0) return fine();
   KV_REQUIRE(x != nullptr && y != nullptr && (rotary == 0 || (positions != nullptr && freq != nullptr)), "null operand");
@@ -146,9 +156,9 @@ inline Verdict check_append(const void *q, const void *q_out, const void *k, con
   KV_PASS(check_heads(tokens, kv_heads, dim, dtype));
   if ((heads + 2 * kv_heads) * dim > MOST) return unsupported("tensor too large");
   KV_PASS(check_rotary(dim, rotary, tokens, heads + 2 * kv_heads));
-  KV_PASS(check_stride(q_token));
-  KV_PASS(check_stride(k_token));
-  KV_PASS(check_stride(v_token));
+  KV_PASS(check_stride(q_token, tokens));
+  KV_PASS(check_stride(k_token, tokens));
+  KV_PASS(check_stride(v_token, tokens));
   KV_PASS(check_rows(tokens, q_out_token, heads * dim));
   KV_PASS(check_pool(num_pages, page_size, kv_heads, dim));
   if (tokens == 0) return fine();
@@ -171,7 +181,7 @@ inline Verdict check_attention(const void *q, const void *k_cache, const void *v
   KV_PASS(check_heads(batch, kv_heads, dim, dtype));
   KV_REQUIRE(heads % kv_heads == 0, "heads must be a multiple of kv_heads");
   if (dim > 256) return unsupported("head_dim above 256");
-  KV_PASS(check_stride(q_stride));
+  KV_PASS(check_stride(q_stride, batch));
   KV_PASS(check_rows(batch, out_stride, heads * dim));
   KV_PASS(check_pool(num_pages, page_size, kv_heads, dim));
   KV_REQUIRE(max_pages >= 0 && max_length >= 0 && window >= 0, "negative size");

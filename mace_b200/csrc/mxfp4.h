@@ -26,7 +26,7 @@ inline kv::Verdict check_tensor(const void *x, const void *codes, const void *sc
   KV_REQUIRE(kv::is_type(dtype), "element type is not MB_F32, MB_F16 or MB_BF16");
   KV_REQUIRE(rows >= 0 && cols >= 0, "negative size");
   if (rows > kv::MOST || cols > kv::MOST - 4096) return kv::unsupported("tensor too large");
-  KV_REQUIRE(stride >= 0 && stride <= kv::MOST_STRIDE && (!written || rows <= 1 || stride >= cols),
+  KV_REQUIRE(stride >= 0 && stride <= kv::MOST_STRIDE && kv::reaches(rows, stride) && (!written || rows <= 1 || stride >= cols),
              "output rows overlap, or stride is negative or too large");
   if (rows == 0 || cols == 0) return kv::fine();
   KV_REQUIRE(x != nullptr && codes != nullptr && scales != nullptr, "null operand");
@@ -40,7 +40,7 @@ inline kv::Verdict check_gemm(const void *a, const void *a_scales, const void *b
   KV_REQUIRE(kv::is_type(dtype), "element type is not MB_F32, MB_F16 or MB_BF16");
   KV_REQUIRE(M >= 0 && N >= 0 && K >= 0, "negative size");
   if (M > kv::MOST - 4096 || N > kv::MOST - 4096 || K > (1 << 30)) return kv::unsupported("matrix too large");
-  KV_REQUIRE(stride >= 0 && stride <= kv::MOST_STRIDE && (M <= 1 || stride >= N), "output rows overlap, or stride is negative or too large");
+  KV_REQUIRE(stride >= 0 && stride <= kv::MOST_STRIDE && kv::reaches(M, stride) && (M <= 1 || stride >= N), "output rows overlap, or stride is negative or too large");
   if (M == 0 || N == 0) return kv::fine();
   KV_REQUIRE(c != nullptr && (K == 0 || (a != nullptr && a_scales != nullptr && b != nullptr && b_scales != nullptr)), "null operand");
   KV_REQUIRE(kv::aligned(a, 16) && kv::aligned(a_scales, 16) && kv::aligned(b, 16) && kv::aligned(b_scales, 16) &&

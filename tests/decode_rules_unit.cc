@@ -83,10 +83,55 @@ static void rows_too_many_or_too_long() {
   EXPECT(code(1, 513, 1, memory + 4) == MB_UNSUPPORTED);
 }
 
+// Strides and extents up to the limits: no sum or product of them leaves 64 bits (the program is built with -fsanitize=undefined), and what
+// overlaps or has no address is refused.
+static void strides_at_the_limits() {
+  const int64_t most = INT32_MAX, far = 1ll << 40, rows = (1ll << 31) - 8;
+  const auto rope = [](int64_t tokens, int64_t heads, int64_t dim, int64_t xt, int64_t xh, int64_t yt, int64_t yh) {
+    return kv::check_rope(X, Y, I, reinterpret_cast<const double *>(memory), tokens, heads, dim, dim, xt, xh, yt, yh, MB_BF16).code;
+  };
+  EXPECT(rope(2, 2, 64, 128, 64, 128, 64) == MB_SUCCESS);
+  EXPECT(rope(2, 2, 64, 128, 64, 64, 128) == MB_SUCCESS);
+  EXPECT(rope(2, 2, 64, 128, 64, 127, 64) == MB_INVALID_ARGS);
+  EXPECT(rope(3, 2, 64, 128, 64, 64, 191) == MB_INVALID_ARGS);
+  EXPECT(rope(3, 2, 64, 128, 64, 64, 192) == MB_SUCCESS);
+  EXPECT(rope(2, 2, 64, 128, 64, far, 64) == MB_SUCCESS);
+  EXPECT(rope(2, 2, 64, 0, 0, 64, far) == MB_SUCCESS);
+  EXPECT(rope(2, 2, 64, 0, 0, far + 1, 64) == MB_INVALID_ARGS);
+  // (heads - 1) * y_head alone would be 2^71
+  EXPECT(rope(2, most / 2, 2, 0, 0, far, far) == MB_INVALID_ARGS);
+  EXPECT(rope(most, 1, 2, far, 2, 2, 2) == MB_INVALID_ARGS);
+  EXPECT(rope(most, 1, 2, 2, 2, far, 2) == MB_INVALID_ARGS);
+  EXPECT(rope(1, most / 2, 2, 2, far, 2, 2) == MB_INVALID_ARGS);
+  EXPECT(rope(1 << 19, 2, 2, far, 2, far, 2) == MB_SUCCESS);
+  EXPECT(rope((1 << 19) + 2, 2, 2, far, 2, far, 2) == MB_INVALID_ARGS);
+  for (const int64_t tokens : {1ll, 2ll, 1ll << 19, 1ll << 31})
+    for (const int64_t heads : {1ll, 2ll, 1ll << 20, 1ll << 30})
+      for (const int64_t a : {0ll, 1ll, 64ll, 1ll << 31, 1ll << 40, (1ll << 62)})
+        for (const int64_t b : {0ll, 2ll, 64ll, 1ll << 20, 1ll << 40, (1ll << 62)}) rope(tokens, heads, 2, a, b, b, a);
+  const auto append = [](int64_t tokens, int64_t q, int64_t q_out, int64_t k, int64_t v) {
+    return kv::check_append(X, Y, X, X, Y, Y, I, I, reinterpret_cast<const double *>(memory), tokens, 1, 1, 8, 8, q, q_out, k, v, 10, 16, MB_F16).code;
+  };
+  EXPECT(append(1 << 19, far, far, far, far) == MB_SUCCESS);
+  for (int i = 0; i < 4; ++i) EXPECT(append(rows, i == 0 ? far : 8, i == 1 ? far : 8, i == 2 ? far : 8, i == 3 ? far : 8) == MB_INVALID_ARGS);
+  const auto attention = [](int64_t batch, int64_t q, int64_t out, int64_t kv_heads, int64_t pages, int64_t page) {
+    return kv::check_attention(X, X, X, I, I, Y, nullptr, nullptr, nullptr, batch, kv_heads, kv_heads, 8, q, out, pages, page, 4, 64, 0, 0, MB_F16).code;
+  };
+  EXPECT(attention(1 << 19, far, far, 1, 10, 16) == MB_SUCCESS);
+  EXPECT(attention(1 << 28, far, 8, 1, 10, 16) == MB_INVALID_ARGS);
+  EXPECT(attention(1 << 28, 8, far, 1, 10, 16) == MB_INVALID_ARGS);
+  EXPECT(attention(1, 8, 8, 1 << 27, 1 << 20, 1 << 10) == MB_UNSUPPORTED);   // a pool of 2^60 values
+  EXPECT(attention(1, 8, 8, 1 << 27, 1 << 20, 1 << 9) == MB_SUCCESS);
+  EXPECT(mx::check_tensor(X, X, X, rows, 32, far, MB_F16, false).code == MB_INVALID_ARGS);
+  EXPECT(mx::check_tensor(X, X, X, 1 << 19, 32, far, MB_F16, true).code == MB_SUCCESS);
+  EXPECT(mx::check_gemm(X, X, X, X, nullptr, Y, (1ll << 31) - 5000, 32, 32, far, MB_F16).code == MB_INVALID_ARGS);
+}
+
 int main() {
   clusters();
   weights_of_too_many_slots();
   rows_too_many_or_too_long();
+  strides_at_the_limits();
   if (failures != 0) std::printf("%d failures\n", failures);
   return failures != 0;
 }
