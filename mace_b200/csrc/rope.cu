@@ -243,6 +243,8 @@ int mb_rope_frequencies(int scaling, int64_t rotary_dim, double base, double fac
       double kept;
       if (scaling == MB_ROPE_BANDS)
         kept = (original_length * f / (2.0 * pi) - low) / (high - low);
+      else if (last < first)   // (every pair turns less than `low` times, or every one more than `high` times)
+        kept = last < 0.0 ? 0.0 : 1.0;
       else
         kept = 1.0 - (static_cast<double>(i) - first) / (last - first);
       kept = std::fmin(std::fmax(kept, 0.0), 1.0);
