@@ -22,6 +22,7 @@ int mb_check_cuda(mb_context *ctx, cudaError_t e, const char *what) {
   if (e == cudaSuccess) return MB_SUCCESS;
   const int code =
       (e == cudaErrorMemoryAllocation) ? MB_OUT_OF_RESOURCES : MB_RUNTIME_ERROR;
+  cudaGetLastError();  // told here: not the error of a launch behind this call
   return mb_fail(ctx, code, "%s: %s", what, cudaGetErrorString(e));
 }
 

@@ -1,0 +1,47 @@
+"""What a failed call of a decode-step operator leaves behind: nothing."""
+import numpy as np
+import pytest
+import torch
+
+from decode_ref import Values
+from test_gpu_decode_attention import Case
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    import mace_b200
+    c = mace_b200.Context(0)
+    yield c
+    c.close()
+
+
+def test_scratch_that_cannot_be_had_is_not_the_next_calls_error(ctx):
+    """Attention with weights wants 4 bytes per query head and slot; more than the device has is refused, and the calls behind it are as
+    they were (one of them asks the runtime for the last error after its launch)."""
+    from mace_b200 import MaceB200Error
+    c = Case(ctx, "bf16", [100, 3], 8, 2, 64, 16, seed=1)
+    length = 1 << 28
+    with pytest.raises(MaceB200Error) as e:   # 2^4 sequences x 2^8 heads x 2^28 slots: 4 TiB (no pointer is followed before that)
+        ctx.paged_attention(c.dq, c.dk, c.dv, c.dt, c.dn, c.out, 16, 256, 256, 64, c.pages, 16, length // 16, length, 1.0, 2, weights_out=c.w_out,
+                            weights_stride=length)
+    assert e.value.code == 2
+    x = np.arange(96 * 40, dtype=np.float32).reshape(1, 96, 40)
+    dx, dy = ctx.upload(x), ctx.alloc(x.nbytes)
+    ctx.transpose2d_batched(dx, dy, 1, 96, 40, 4)
+    ctx.sync()
+    assert np.array_equal(ctx.download(dy, (1, 40, 96), np.float32), x.transpose(0, 2, 1))
+    c.run().check()
+
+
+def test_memory_that_cannot_be_had_is_not_the_next_calls_error(ctx):
+    from mace_b200 import MaceB200Error
+    with pytest.raises(MaceB200Error) as e:
+        ctx.alloc(1 << 42)
+    assert e.value.code == 2
+    x = np.arange(64, dtype=np.float32).reshape(1, 8, 8)
+    dx, dy = ctx.upload(x), ctx.alloc(x.nbytes)
+    ctx.transpose2d_batched(dx, dy, 1, 8, 8, 4)
+    ctx.sync()
+    assert np.array_equal(ctx.download(dy, (1, 8, 8), np.float32), x.transpose(0, 2, 1))
