@@ -538,8 +538,8 @@ int mb_rope_kv_append(mb_context *ctx, const void *q, void *q_out,
                       int dtype);
 
 /* Attention of one new token per sequence over the paged cache.  q and out
- * [batch][heads][head_dim], token strides in elements; kv head h serves query
- * heads h * heads / kv_heads .. (h + 1) * heads / kv_heads - 1.
+ * [batch][heads][head_dim], token strides in elements (out == q allowed, then
+ * with the same stride); kv head h serves query heads h * heads / kv_heads .. (h + 1) * heads / kv_heads - 1.
  *   s_j = scale * q . k_j,  p_j = exp(s_j - lse),  out = sum_j p_j v_j
  * over the slots j < lengths[b], or with window > 0 the last `window` of them.
  * lse (may be NULL): [batch][heads].  A sequence of length 0 gives out = 0 and

@@ -199,6 +199,8 @@ inline Verdict check_attention(const void *q, const void *k_cache, const void *v
   const uintptr_t size = type_bytes(dtype);
   KV_REQUIRE(aligned(q, size) && aligned(out, size) && aligned(k_cache, size) && aligned(v_cache, size) && aligned(table, 4) &&
              aligned(lengths, 4) && aligned(lse, 4) && aligned(weights_in, 4) && aligned(weights_out, 4), "misaligned operand");
+  // (a head's result is written when all blocks that read its query have: another sequence's may still be read)
+  KV_REQUIRE(q != out || batch <= 1 || q_stride == out_stride, "in place with another stride");
   return fine();
 }
 

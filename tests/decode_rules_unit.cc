@@ -127,7 +127,18 @@ static void strides_at_the_limits() {
   EXPECT(mx::check_gemm(X, X, X, X, nullptr, Y, (1ll << 31) - 5000, 32, 32, far, MB_F16).code == MB_INVALID_ARGS);
 }
 
+static void attention_in_place() {
+  const auto code = [](const void *out, int64_t batch, int64_t q_stride, int64_t out_stride) {
+    return kv::check_attention(X, X, X, I, I, out, nullptr, nullptr, nullptr, batch, 8, 2, 64, q_stride, out_stride, 10, 16, 4, 64, 0, 0, MB_F16).code;
+  };
+  EXPECT(code(X, 2, 512, 512) == MB_SUCCESS);
+  EXPECT(code(X, 2, 1024, 512) == MB_INVALID_ARGS);
+  EXPECT(code(X, 1, 1024, 512) == MB_SUCCESS);
+  EXPECT(code(Y, 2, 1024, 512) == MB_SUCCESS);
+}
+
 int main() {
+  attention_in_place();
   clusters();
   weights_of_too_many_slots();
   rows_too_many_or_too_long();

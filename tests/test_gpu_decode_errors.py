@@ -45,3 +45,23 @@ def test_memory_that_cannot_be_had_is_not_the_next_calls_error(ctx):
     ctx.transpose2d_batched(dx, dy, 1, 8, 8, 4)
     ctx.sync()
     assert np.array_equal(ctx.download(dy, (1, 8, 8), np.float32), x.transpose(0, 2, 1))
+
+
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("lengths,heads,kv_heads,dim,page", [([500, 3, 0, 1000], 8, 2, 64, 16), ([30000, 77], 40, 1, 128, 20), ([9000] * 6, 64, 4, 128, 16),
+                                                             ([700] * 3, 6, 2, 50, 16), ([20] * 1100, 4, 2, 64, 16)])
+def test_attention_in_place(ctx, name, lengths, heads, kv_heads, dim, page):
+    """out == q, on clusters, as runs and in one block: heads are written when no block reads their queries any more."""
+    c = Case(ctx, name, lengths, heads, kv_heads, dim, page, seed=3)
+    for _ in range(3):
+        c.out = c.dq = Values(ctx, c.q)
+        c.run().check()
+
+
+def test_attention_in_place_with_another_stride_is_refused(ctx):
+    from mace_b200 import MaceB200Error
+    c = Case(ctx, "bf16", [20, 33], 4, 2, 64, 16)
+    c.out = c.dq
+    with pytest.raises(MaceB200Error) as e:
+        c.run(q_stride=300)
+    assert e.value.code == 1 and "in place" in str(e.value)
