@@ -69,6 +69,7 @@ inline bool aligned(const void *p, uintptr_t to) { return reinterpret_cast<uintp
 // Extents above these are refused, so that counts fit 31 bits and byte offsets 63 (a tensor's two strides together).
 constexpr int64_t MOST = INT32_MAX;
 constexpr int64_t MOST_DIM = 1 << 16;   // rotary head_dim
+constexpr int64_t MOST_SLOTS = MOST - (1 << 16);   // of a sequence: an index that steps past the last by a cluster's threads (16 x 1024) fits
 constexpr int64_t MOST_STRIDE = 1ll << 40, MOST_OFFSET = 1ll << 59;
 
 #define KV_REQUIRE(cond, why) \
@@ -185,7 +186,7 @@ inline Verdict check_attention(const void *q, const void *k_cache, const void *v
   KV_PASS(check_rows(batch, out_stride, heads * dim));
   KV_PASS(check_pool(num_pages, page_size, kv_heads, dim));
   KV_REQUIRE(max_pages >= 0 && max_length >= 0 && window >= 0, "negative size");
-  if (max_pages > MOST / page_size || max_length > MOST - 4096) return unsupported("more than 2^31 - 4096 slots");
+  if (max_pages > MOST / page_size || max_length > MOST_SLOTS) return unsupported("more than 2^31 - 2^16 - 1 slots");
   if (batch * heads > MOST / 4) return unsupported("too many query heads");
   KV_REQUIRE(weights_in == nullptr || weights_out != nullptr, "weights_in without weights_out");
   KV_REQUIRE(weights_out == nullptr || (weights_stride >= longest_of(max_length, max_pages, page_size) && weights_stride <= MOST),
@@ -231,8 +232,8 @@ inline Verdict check_evict(const void *k_src, const void *v_src, const int32_t *
   KV_REQUIRE(src_max_pages >= 0 && dst_max_pages >= 0 && max_length >= 0, "negative size");
   KV_REQUIRE(budget >= 1 && sinks >= 0 && recent >= 0 && sinks <= budget && recent <= budget - sinks,
              "budget must be at least 1 and at least sinks + recent");
-  if (src_max_pages > MOST / page_size || dst_max_pages > MOST / page_size || max_length > MOST - 4096 || budget > MOST - 4096)
-    return unsupported("more than 2^31 - 4096 slots");
+  if (src_max_pages > MOST / page_size || dst_max_pages > MOST / page_size || max_length > MOST_SLOTS || budget > MOST_SLOTS)
+    return unsupported("more than 2^31 - 2^16 - 1 slots");
   const int64_t longest = longest_of(max_length, src_max_pages, page_size), stays = budget < longest ? budget : longest;
   KV_REQUIRE(dst_max_pages * page_size >= stays, "the destination's table has no room for budget slots");
   KV_REQUIRE(weights_stride >= longest && weights_stride <= MOST, "weights_stride below the longest sequence, or too large");

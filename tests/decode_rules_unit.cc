@@ -21,8 +21,7 @@ static void clusters() {
       for (const int most : {8, 16})
         for (const int64_t bytes : {4, 256, 512, 1024, 2048})
           for (const int64_t units : {1ll, 2ll, 3ll, 7ll, 8ll, 9ll, 18ll, 19ll, 37ll, 74ll, 75ll, 148ll, 149ll, 1ll << 29})
-            for (const int64_t longest : {0ll, 1ll, 127ll, 128ll, 129ll, 1000ll, 2048ll, 2049ll, 8192ll, 16384ll, 16385ll, 30000ll, 120000ll,
-                                          (1ll << 31) - 4097}) {
+            for (const int64_t longest : {0ll, 1ll, 127ll, 128ll, 129ll, 1000ll, 2048ll, 2049ll, 8192ll, 16384ll, 16385ll, 30000ll, 120000ll, (1ll << 31) - 65537}) {
               const int c = kv::cluster_of(units, longest, bytes, most, share, r);
               EXPECT(c >= 1 && c <= most && (c & (c - 1)) == 0);
               if (c == 1) continue;
@@ -137,7 +136,25 @@ static void attention_in_place() {
   EXPECT(code(Y, 2, 1024, 512) == MB_SUCCESS);
 }
 
+// Eviction's threads step through a sequence's first and last slots by as many as a cluster has, in 32 bits.
+static void sequences_of_almost_2_31() {
+  const int64_t most = kv::MOST_SLOTS;
+  EXPECT(most + 16 * 1024 <= INT32_MAX);
+  const auto evict = [](int64_t length, int64_t budget, int64_t sinks, int64_t recent) {
+    return kv::check_evict(X, X, I, I, F, Y, Y, I, I, reinterpret_cast<const float *>(uintptr_t{1} << 45), I, 1, 1, 1, 1 << 16, (1 << 15) - 1, (1 << 15) - 1,
+                           (1 << 15) - 1, (1 << 15) - 1, length, length, budget, sinks, recent, MB_F16, budget).code;
+  };
+  EXPECT(evict(most, most, most, 0) == MB_SUCCESS);
+  EXPECT(evict(most, most, 0, most) == MB_SUCCESS);
+  EXPECT(evict(INT32_MAX - 4096, 10, 0, 0) == MB_UNSUPPORTED);
+  EXPECT(evict(1000, INT32_MAX - 4096, INT32_MAX - 4096, 0) == MB_UNSUPPORTED);
+  EXPECT(evict(1000, most + 1, 0, most + 1) == MB_UNSUPPORTED);
+  EXPECT(kv::check_attention(X, X, X, I, I, Y, nullptr, nullptr, nullptr, 1, 1, 1, 8, 8, 8, 10, 1 << 16, 1 << 14, most + 1, 0, 0, MB_F16).code == MB_UNSUPPORTED);
+  EXPECT(kv::check_attention(X, X, X, I, I, Y, nullptr, nullptr, nullptr, 1, 1, 1, 8, 8, 8, 10, 1 << 16, 1 << 14, most, 0, 0, MB_F16).code == MB_SUCCESS);
+}
+
 int main() {
+  sequences_of_almost_2_31();
   attention_in_place();
   clusters();
   weights_of_too_many_slots();
