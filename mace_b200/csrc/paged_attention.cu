@@ -1119,7 +1119,8 @@ extern "C" int mb_paged_attention(mb_context *ctx, const void *q, const void *k_
   p.status = ctx->dev_status;
 
   const bool f32 = dtype == MB_F32;
-  const bool by_mma = ctx->use_tensor_cores && head_dim % (f32 ? 4 : 8) == 0 && (!f32 || head_dim <= 128) && kv::aligned(k_cache, 16) &&
+  // (a pool without pages has no address that a copy of no bytes could name)
+  const bool by_mma = ctx->use_tensor_cores && num_pages > 0 && head_dim % (f32 ? 4 : 8) == 0 && (!f32 || head_dim <= 128) && kv::aligned(k_cache, 16) &&
                       kv::aligned(v_cache, 16);
   // Rows of a block: as many of a group's heads as registers hold, since every block of heads reads the run again (20 heads of 128 in one
   // block of 24 142 us, in two of 16 171).

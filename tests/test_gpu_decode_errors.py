@@ -1,4 +1,6 @@
 """What a failed call of a decode-step operator leaves behind: nothing."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -45,6 +47,27 @@ def test_memory_that_cannot_be_had_is_not_the_next_calls_error(ctx):
     ctx.transpose2d_batched(dx, dy, 1, 8, 8, 4)
     ctx.sync()
     assert np.array_equal(ctx.download(dy, (1, 8, 8), np.float32), x.transpose(0, 2, 1))
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_attention_over_a_pool_without_pages(ctx, name):
+    """Null pools: empty sequences are served, others have pages that are not there."""
+    from mace_b200 import MaceB200Error
+    c = Case(ctx, name, [40, 0, 700], 8, 2, 64, 16, seed=6)
+
+    class Nowhere:
+        ptr = None
+    c.dk = c.dv = Nowhere
+    c.pages = 0
+    with pytest.raises(MaceB200Error) as e:
+        c.run()
+    assert e.value.code == 4 and "outside its range" in str(e.value)
+    assert (c.out.get() == 0).all() and (c.lse.get() == -math.inf).all()
+    for b, n in enumerate(c.lengths):
+        assert np.array_equal(c.w_out.get().numpy()[b, :, :n], c.w_in[b, :, :n])
+    c.dn = ctx.upload(np.zeros(3, np.int32))
+    c.run()
+    assert (c.out.get() == 0).all()
 
 
 @pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
