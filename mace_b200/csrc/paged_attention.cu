@@ -898,15 +898,14 @@ __global__ void __launch_bounds__(THREADS, DIM * sizeof(T) == 128 && HEADS == 2 
       }
       __syncwarp();
     } else {
-      // (raised in the exponent: the 2^-20 that this costs them is less than what a pair of 16-bit values does)
       uint32_t least = 0xffffffffu;   // the smallest probability's bits less one: zeros come last
 #pragma unroll
       for (int t = 0; t < HEADS; ++t) {
-        const float m0 = top[t][0] == -INFINITY ? 0.f : top[t][0] - LIFT<T>, m1 = top[t][1] == -INFINITY ? 0.f : top[t][1] - LIFT<T>;
+        const float m0 = top[t][0] == -INFINITY ? 0.f : top[t][0], m1 = top[t][1] == -INFINITY ? 0.f : top[t][1];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          s[t][2 * i] = exp2f(s[t][2 * i] - m0);
-          s[t][2 * i + 1] = exp2f(s[t][2 * i + 1] - m1);
+          s[t][2 * i] = exp2f(s[t][2 * i] - m0) * RAISED<T>;
+          s[t][2 * i + 1] = exp2f(s[t][2 * i + 1] - m1) * RAISED<T>;
           sum[t][0] += s[t][2 * i];
           sum[t][1] += s[t][2 * i + 1];
           if (HALVES) least = min(least, min(__float_as_uint(s[t][2 * i]) - 1u, __float_as_uint(s[t][2 * i + 1]) - 1u));
