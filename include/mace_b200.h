@@ -467,7 +467,9 @@ int mb_histogram_f32(mb_context *ctx, const float *in, int64_t size, float min_v
  *
  * Element types (DT_FLOAT, DT_HALF and DT_BFLOAT16 of the reference): values of
  * the 16-bit types are widened to fp32, every sum is kept in fp32, results are
- * rounded once, to nearest even.
+ * rounded once, to nearest even.  (On the tensor cores attention multiplies
+ * probabilities that are exact to 2^-16 whatever their size, and fp32 products
+ * are exact to 2^-20; with the option "tensor_cores" at 0 both are fp32's own.)
  *
  * All calls enqueue on the context's stream and may be captured into a graph
  * (mb_graph_begin; run the sequence once uncaptured first, as ever).  Indices
@@ -510,7 +512,7 @@ int mb_rope_frequencies(int scaling, int64_t rotary_dim, double base,
  * inverse turns the other way, which is the gradient with respect to x.  The
  * angle is formed and reduced in 64 bits.  y == x with the same strides is
  * allowed, other overlaps are not.  freq: device memory, rotary_dim / 2
- * doubles. */
+ * doubles.  rotary_dim up to 12288. */
 int mb_rope(mb_context *ctx, const void *x, void *y, const int32_t *positions,
             const double *freq, int64_t tokens, int64_t heads, int64_t head_dim,
             int64_t rotary_dim, int64_t x_token_stride, int64_t x_head_stride,
@@ -553,8 +555,10 @@ int mb_rope_kv_append(mb_context *ctx, const void *q, void *q_out,
  * weights_out is allowed) plus the sum of p_j over the query heads that kv
  * head h serves; slots outside the window receive weights_in alone, entries
  * from lengths[b] on stay as they are; the call then takes
- * 4 * batch * heads * max_length bytes of scratch.  head_dim up to 256.  An infinite
- * value (not key) in a slot that counts gives NaN or an infinity. */
+ * 4 * batch * heads * max_length bytes of scratch.  head_dim up to 256, up to
+ * 2^31 - 2^16 - 1 slots.  An infinite value (not key) in a slot that counts
+ * gives NaN or an infinity; finite ones, up to the type's largest, a finite
+ * result (up to 2^24 slots of the heaviest one's weight). */
 int mb_paged_attention(mb_context *ctx, const void *q, const void *k_cache,
                        const void *v_cache, const int32_t *page_table,
                        const int32_t *lengths, void *out, float *lse,
@@ -573,7 +577,8 @@ int mb_paged_attention(mb_context *ctx, const void *q, const void *k_cache,
  * in order and is copied to slots 0, 1, ... of the destination: pages of
  * k_dst / v_dst named by dst_table (the pools may be the source pools, the
  * pages may not be pages that the call reads, and no page may be named twice;
- * source pages may be shared between sequences).  Device memory is written as
+ * source pages may be shared between sequences; up to 2^31 - 2^16 - 1 slots).
+ * Device memory is written as
  * follows, all of it only up to the new length min(lengths[b], budget):
  *   dst_lengths [batch]                     the new lengths (may be lengths)
  *   dst_weights [batch][kv_heads][budget]   the weights of the kept slots
