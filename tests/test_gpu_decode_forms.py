@@ -75,3 +75,35 @@ def test_sums_over_a_long_run(ctx, name, length):
     assert ((lse.get().double() - math.log(length)).abs() <= 2 * chunks * 2.0 ** -24 + 2.0 ** -20).all()
     for x in (dq, dk, dv, out, lse, table, lengths):
         x.free()
+
+
+def test_two_graphs_share_scratch(ctx):
+    """Captured steps of different sizes, one recorded before the scratch memory grew, replayed in turn with eager calls in between."""
+    import ctypes as C
+
+    from mace_b200.capi import lib
+    L = lib()
+    cases = [Case(ctx, "bf16", [3000, 5, 0], 8, 2, 128, 16, seed=1), Case(ctx, "f16", [9000] * 5, 32, 8, 128, 16, seed=2),
+             Case(ctx, "f32", [1200, 700], 6, 3, 50, 16, seed=3)]
+    graphs = []
+    for c in cases:
+        c.run()
+        assert L.mb_graph_begin(ctx.h) == 0
+        c.call()
+        graph = C.c_void_p()
+        assert L.mb_graph_end(ctx.h, C.byref(graph)) == 0
+        graphs.append(graph)
+    for _ in range(3):
+        for c, graph in zip(cases, graphs):
+            for v in (c.out, c.lse):
+                ctx.h2d(v.buf, np.full(v.nbytes, 0x7f, np.uint8))
+            ctx.h2d(c.w_out.buf, np.full(c.w_out.shape, -5.0, np.float32))
+            ctx.sync()
+        for graph in graphs[::-1] + graphs:
+            assert L.mb_graph_launch(ctx.h, graph) == 0
+        cases[0].call()
+        ctx.sync()
+        for c in cases:
+            c.check()
+    for graph in graphs:
+        L.mb_graph_destroy(ctx.h, graph)
