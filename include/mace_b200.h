@@ -557,8 +557,9 @@ int mb_rope_kv_append(mb_context *ctx, const void *q, void *q_out,
  * from lengths[b] on stay as they are; the call then takes
  * 4 * batch * heads * max_length bytes of scratch.  head_dim up to 256, up to
  * 2^31 - 2^16 - 1 slots.  An infinite value (not key) in a slot that counts
- * gives NaN or an infinity; finite ones, up to the type's largest, a finite
- * result (up to 2^24 slots of the heaviest one's weight). */
+ * gives NaN or an infinity; finite ones, whatever their sum would be, a finite
+ * result (of up to 2^24 slots of the heaviest one's weight, and unless a
+ * rounding passes the type's largest). */
 int mb_paged_attention(mb_context *ctx, const void *q, const void *k_cache,
                        const void *v_cache, const int32_t *page_table,
                        const int32_t *lengths, void *out, float *lse,
