@@ -527,7 +527,7 @@ int mb_rope(mb_context *ctx, const void *x, void *y, const int32_t *positions,
  * cache (padding of a batch); q is rotated all the same.  Token strides in
  * elements, heads contiguous (q, k and v may be parts of one row).  Slots that
  * are not negative must differ from one another; what a slot named twice
- * holds is not defined. */
+ * holds is not defined.  rotary_dim up to 12286. */
 int mb_rope_kv_append(mb_context *ctx, const void *q, void *q_out,
                       const void *k, const void *v, void *k_cache,
                       void *v_cache, const int32_t *positions,
@@ -586,7 +586,9 @@ int mb_paged_attention(mb_context *ctx, const void *q, const void *k_cache,
  *   kept        [batch][kv_heads][budget]   their old slots, ascending; here
  *                                           entries from the new length on
  *                                           become -1
- * weights: [batch][kv_heads][weights_stride].  sinks + recent <= budget.
+ * weights: [batch][kv_heads][weights_stride].  sinks + recent <= budget.  A row
+ * of head_dim values is copied in words of 16, 4 or 2 bytes, the most that it
+ * and the four pools' addresses are multiples of, and has at most 512 of them.
  *
  * mb_kv_evict_strided: the same with dst_weights [batch][kv_heads]
  * [dst_weights_stride], dst_weights_stride >= budget, whose entries from the

@@ -175,7 +175,7 @@ int launch(mb_context *ctx, RopeParams &p, int heads) {
   if (rows > 65535) return mb_fail(ctx, MB_UNSUPPORTED, "mb_rope: a token has too many values");
   fast_div_make(p.half, &p.half_mul, &p.half_shift);
   const size_t smem = (sizeof(float2) * p.half + (p.slots != nullptr ? sizeof(int64_t) : 0)) * p.tokens_per_block;
-  if (smem > (48u << 10)) return mb_fail(ctx, MB_UNSUPPORTED, "mb_rope: rotary_dim above 12288");
+  if (smem > (48u << 10)) return mb_fail(ctx, MB_UNSUPPORTED, "mb_rope: rotary_dim too large for a block's table of sines");
   MB_CUDA(ctx, mb_launch_chained(ctx, rope_kernel<T, V, INTERLEAVED>, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(rows)),
                                  dim3(THREADS), smem, p));
   ctx->launches++;

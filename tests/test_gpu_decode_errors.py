@@ -88,3 +88,46 @@ def test_attention_in_place_with_another_stride_is_refused(ctx):
     with pytest.raises(MaceB200Error) as e:
         c.run(q_stride=300)
     assert e.value.code == 1 and "in place" in str(e.value)
+
+
+def test_the_widest_rotation(ctx):
+    """rotary_dim as large as the header allows, and one pair more."""
+    from decode_ref import TYPES, tensor, turn
+    from mace_b200 import MaceB200Error
+    from test_gpu_decode_rope import _check, _freq
+    rng = np.random.default_rng(9)
+    name, tokens = "f32", 2
+    for rotary, append in ((12288, False), (12290, False), (12286, True), (12288, True)):
+        x = tensor(rng, name, tokens, 1, rotary)
+        positions = np.array([3, 100000], np.int32)
+        dx, dy, dp, df = Values(ctx, x), Values(ctx, x), ctx.upload(positions), ctx.upload(_freq(rotary))
+        pools = [ctx.alloc(2 * rotary * 4) for _ in range(2)]
+
+        def call():
+            if append:
+                ctx.rope_kv_append(dx, dy, dx, dx, *pools, dp, ctx.upload(np.array([1, 0], np.int32)), df, tokens, 1, 1, rotary, rotary, 1, 2, TYPES[name][0])
+            else:
+                ctx.rope(dx, dy, dp, df, tokens, 1, rotary, rotary, TYPES[name][0])
+            ctx.sync()
+        if rotary == (12288 if append else 12290):
+            with pytest.raises(MaceB200Error) as e:
+                call()
+            assert e.value.code == 3
+            continue
+        call()
+        want, size = turn(x, positions, _freq(rotary), 1.0, rotary, False)
+        _check(dy.get(), want, size, name)
+
+
+@pytest.mark.parametrize("name,dim,code", [("bf16", 511, 0), ("bf16", 512, 0), ("bf16", 513, 3), ("f32", 513, 3), ("bf16", 4096, 0), ("bf16", 4104, 3)])
+def test_the_widest_rows_of_eviction(ctx, name, dim, code):
+    from mace_b200 import MaceB200Error
+    from test_gpu_decode_evict import _case
+    run, check = _case(ctx, name, [30, 9], 1, dim, 4, 10, 1, 2, seed=dim)
+    if code:
+        with pytest.raises(MaceB200Error) as e:
+            run()
+        assert e.value.code == code
+    else:
+        run()
+        check()
